@@ -727,6 +727,45 @@ UGB_API int32_t ugb_selective_step(ugb_device *dev, const ugb_slice *x, const ug
                                    ugb_slice *state, ugb_slice *out, size_t rows, size_t channels, size_t rank, size_t states,
                                    float scale);
 
+/* ------------------------------------------------ generation beyond greedy steps */
+/* A token per row of logits, from given random numbers.  logits F32 or BF16 [rows], ld elements apart: [vocab]
+ * (vocab <= 262144).  With w_i = exp((x_i - max x) / temperature) and the tokens in the order of falling logits (equal
+ * ones by index): the first top_k stay (0: all); of these the shortest beginning whose weights reach top_p of
+ * theirs (>= 1: all); of these the ones with w_i >= min_p.  The token is the first one, by index, at which the running sum
+ * of what stays exceeds u times its total; temperature 0 takes the best one, the first of equal ones.  temperature,
+ * top_p, min_p, u F32 [rows], top_k I32 [rows], all but u null for 1, off, off, off; tokens I32 [rows]; prob
+ * F32 [rows] or null: the chosen token's share of what stayed.  NaN and -inf are no candidates, a row of nothing
+ * else gives token -1 and prob 0; +inf beats every finite logit.  Sums are exact integers: the same
+ * row gives the same token in any batch.  A parameter outside its range (temperature >= 0 and finite, top_k >= 0,
+ * top_p > 0, 0 <= min_p <= 1, 0 <= u < 1) is UGB_ERR_INVALID at the next ugb_sync, and its row is left as it was. */
+UGB_API int32_t ugb_sample(ugb_device *dev, const ugb_slice *logits, const ugb_slice *temperature, const ugb_slice *top_k,
+                           const ugb_slice *top_p, const ugb_slice *min_p, const ugb_slice *u, ugb_slice *tokens, ugb_slice *prob,
+                           size_t rows, size_t vocab, size_t ld);
+/* The same over the logits of a model's last step or prompt: the tokens become what ugb_llama_decode(m, NULL, n) /
+ * ugb_hybrid_decode feeds next and what UGB_*_NEXT_TOKENS reads, in place of the greedy ones.  A tensor-parallel rank
+ * holds a part of the vocabulary only: UGB_ERR_UNSUPPORTED. */
+UGB_API int32_t ugb_llama_sample(ugb_llama *m, const ugb_slice *temperature, const ugb_slice *top_k, const ugb_slice *top_p,
+                                 const ugb_slice *min_p, const ugb_slice *u, ugb_slice *prob);
+UGB_API int32_t ugb_hybrid_sample(ugb_hybrid *m, const ugb_slice *temperature, const ugb_slice *top_k, const ugb_slice *top_p,
+                                  const ugb_slice *min_p, const ugb_slice *u, ugb_slice *prob);
+
+/* Drafted nodes.  Sequence s has pos[s] committed positions (pos I32 [b]) and t <= 128 drafted nodes behind them, node i in
+ * cache row pos[s] + i whatever its depth.  parents I32 [b, t]: -1 (follows the committed positions) or an earlier node.
+ * pos[s] = -1: there is no sequence in this place, and nothing of it is read or written; any other position whose rows leave
+ * the cache, or a parent that is no earlier node, is UGB_ERR_INVALID at the next ugb_sync, and the sequence is left as it was. */
+/* ugb_head_inputs for drafted nodes: rotary position pos[s] + number of the node's ancestors, cache row pos[s] + i.  dim and
+ * vdim at most 256; the rest as there. */
+UGB_API int32_t ugb_tree_inputs(ugb_device *dev, const ugb_slice *pre, const ugb_slice *cos_, const ugb_slice *sin_,
+                                const ugb_slice *pos, const ugb_slice *parents, ugb_slice *q, ugb_slice *kcache, ugb_slice *vcache,
+                                size_t b, size_t t, size_t heads, size_t kv_heads, size_t dim, size_t vdim, size_t rot_dims,
+                                int32_t interleaved, int32_t qk_norm, float eps, size_t t_max);
+/* Moves the rows of accepted nodes up behind the committed ones: row pos[s] + path[s, i] of every head of k and v to row
+ * pos[s] + i for i < count[s].  k, v T [b, kv_heads, t_max, dq / dv], path I32 [b, most], count I32 [b], most <= 128; the nodes of
+ * a path ascend (as along any way down a tree); every other row stays as it was.  A count above most, a path that does
+ * not ascend or leaves the cache: UGB_ERR_INVALID at the next ugb_sync, and the sequence is left as it was. */
+UGB_API int32_t ugb_cache_keep(ugb_device *dev, ugb_slice *k, ugb_slice *v, const ugb_slice *pos, const ugb_slice *path,
+                               const ugb_slice *count, size_t b, size_t kv_heads, size_t dq, size_t dv, size_t t_max, size_t most);
+
 #ifdef __cplusplus
 }
 #endif

@@ -144,3 +144,14 @@ int32_t engine_read_rows(ugb_engine *m, const void *src, size_t rows, size_t col
   UGB_CUDA(dev, cudaStreamSynchronize(dev->stream));
   return UGB_OK;
 }
+
+int32_t engine_sample(ugb_engine *m, const ugb_slice *temperature, const ugb_slice *top_k, const ugb_slice *top_p, const ugb_slice *min_p,
+                      const ugb_slice *u, ugb_slice *prob) {
+  ugb_device *dev = m->dev;
+  UGB_REQUIRE(dev, m->host_pos > 0, UGB_ERR_INVALID, "sample: no step or prompt has left logits");
+  ugb_slice logits, tokens;
+  logits.dev = tokens.dev = dev;
+  logits.ptr = m->logits; logits.len = (size_t)m->batch * m->logits_ld; logits.dtype = UGB_F32;
+  tokens.ptr = m->next; tokens.len = (size_t)m->batch; tokens.dtype = UGB_I32;
+  return ugb_sample(dev, &logits, temperature, top_k, top_p, min_p, u, &tokens, prob, (size_t)m->batch, (size_t)m->vl, (size_t)m->logits_ld);
+}

@@ -73,5 +73,8 @@ int32_t engine_put_matrix(ugb_engine *m, const ugb_slice *w, void *dst, int32_t 
 int32_t engine_reset(ugb_engine *m, int32_t pos);
 int32_t engine_decode(ugb_engine *m, const ugb_slice *tokens, int32_t n_steps);
 int32_t engine_prefill(ugb_engine *m, const ugb_slice *tokens, int32_t t, int32_t all_logits);
+// Tokens of the last logits from given random numbers, in place of the greedy ones (sampling.cuh); parameters as in ugb_sample.
+int32_t engine_sample(ugb_engine *m, const ugb_slice *temperature, const ugb_slice *top_k, const ugb_slice *top_p, const ugb_slice *min_p,
+                      const ugb_slice *u, ugb_slice *prob);
 // Blocking host copy of `rows` x `cols` 4-byte elements with a source pitch in elements.
 int32_t engine_read_rows(ugb_engine *m, const void *src, size_t rows, size_t cols, size_t src_ld, void *host_dst, size_t len);

@@ -716,6 +716,11 @@ int32_t ugb_hybrid_decode(ugb_hybrid *m, const ugb_slice *tokens, int32_t n_step
   return m ? engine_decode(m, tokens, n_steps) : UGB_ERR_INVALID;
 }
 
+int32_t ugb_hybrid_sample(ugb_hybrid *m, const ugb_slice *temperature, const ugb_slice *top_k, const ugb_slice *top_p, const ugb_slice *min_p,
+                          const ugb_slice *u, ugb_slice *prob) {
+  return m ? engine_sample(m, temperature, top_k, top_p, min_p, u, prob) : UGB_ERR_INVALID;
+}
+
 int32_t ugb_hybrid_prefill(ugb_hybrid *m, const ugb_slice *tokens, int32_t t, int32_t all_logits) {
   return m ? engine_prefill(m, tokens, t, all_logits) : UGB_ERR_INVALID;
 }

@@ -950,6 +950,13 @@ int32_t ugb_llama_decode(ugb_llama *m, const ugb_slice *tokens, int32_t n_steps)
   return m ? engine_decode(m, tokens, n_steps) : UGB_ERR_INVALID;
 }
 
+int32_t ugb_llama_sample(ugb_llama *m, const ugb_slice *temperature, const ugb_slice *top_k, const ugb_slice *top_p, const ugb_slice *min_p,
+                         const ugb_slice *u, ugb_slice *prob) {
+  if (!m) return UGB_ERR_INVALID;
+  UGB_REQUIRE(m->dev, m->tp_size == 1, UGB_ERR_UNSUPPORTED, "sample: rank %d of %d holds a part of the vocabulary", m->tp_rank, m->tp_size);
+  return engine_sample(m, temperature, top_k, top_p, min_p, u, prob);
+}
+
 int32_t ugb_llama_prefill(ugb_llama *m, const ugb_slice *tokens, int32_t t, int32_t all_logits) {
   return m ? engine_prefill(m, tokens, t, all_logits) : UGB_ERR_INVALID;
 }

@@ -122,6 +122,12 @@ static inline int32_t ugb_check_slice(ugb_device *dev, const ugb_slice *s, int32
     if (rc__ != UGB_OK) return rc__;                                      \
   } while (0)
 
+// Whether two slices share memory.
+static inline bool ugb_overlap(const ugb_slice *a, const ugb_slice *b) {
+  const uintptr_t a0 = (uintptr_t)a->ptr, b0 = (uintptr_t)b->ptr, an = a->len * ugb_dtype_size(a->dtype), bn = b->len * ugb_dtype_size(b->dtype);
+  return an && bn && a0 < b0 + bn && b0 < a0 + an;
+}
+
 // ---- programmatic dependent launch ------------------------------------------
 // A kernel launched with ugb_launch(..., pdl = true) may start while the kernel
 // before it on the stream is still running.  It must execute ugb_pdl_wait()

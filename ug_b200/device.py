@@ -166,6 +166,12 @@ class Device:
         s.copy_host_to_device(values, bf16)
         return s
 
+    def wrap(self, device_ptr, dtype, length):
+        """A slice over ``length`` elements of device memory that the caller owns and keeps (ugb_wrap)."""
+        h = C.c_void_p()
+        self._check(lib.ugb_wrap(self._h, device_ptr, int(dtype), length, C.byref(h)))
+        return Slice(self, h)
+
     def synchronize(self):
         self._check(lib.ugb_sync(self._h))
 
@@ -329,3 +335,21 @@ class Device:
         """One position of the selective scan for every row, step-size projection included."""
         self._check(lib.ugb_selective_step(self._h, x._h, low_bc._h, w_dt._h, z._h, a_log._h, skip._h, dt_bias._h, state._h, out._h,
                                            rows, channels, rank, states, scale))
+
+    # ---- generation beyond greedy steps --------------------------------------
+    def sample(self, logits, u, tokens, rows, vocab, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, ld=None):
+        """A token per row of logits from the random numbers ``u``: temperature, then top-k, top-p and min-p (one value per row
+        each, None = off); rows are ``ld`` elements apart."""
+        opt = lambda s: s._h if s is not None else None
+        self._check(lib.ugb_sample(self._h, logits._h, opt(temperature), opt(top_k), opt(top_p), opt(min_p), u._h, tokens._h, opt(prob),
+                                   rows, vocab, vocab if ld is None else ld))
+
+    def tree_inputs(self, pre, cos, sin, pos, parents, q, kcache, vcache, b, t, heads, kv_heads, dim, vdim, rot_dims, interleaved, qk_norm, eps,
+                    t_max):
+        """:meth:`head_inputs` for drafted nodes: rotary positions by depth, cache rows in the order of the nodes."""
+        self._check(lib.ugb_tree_inputs(self._h, pre._h, cos._h, sin._h, pos._h, parents._h, q._h, kcache._h, vcache._h, b, t, heads, kv_heads,
+                                        dim, vdim, rot_dims, int(interleaved), int(qk_norm), eps, t_max))
+
+    def cache_keep(self, k, v, pos, path, count, b, kv_heads, dq, dv, t_max, most):
+        """Moves the cache rows of accepted nodes up behind the committed positions."""
+        self._check(lib.ugb_cache_keep(self._h, k._h, v._h, pos._h, path._h, count._h, b, kv_heads, dq, dv, t_max, most))

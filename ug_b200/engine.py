@@ -12,7 +12,7 @@ from .device import DType, UgError
 
 
 class EngineModel:
-    """``batch`` independent sequences at one shared position, greedy choice on the device."""
+    """``batch`` independent sequences at one shared position, choice of tokens on the device (greedy, or :meth:`sample`)."""
 
     PREFIX = None
     _fed = []      # tokens of steps whose copies may be on their way
@@ -104,6 +104,21 @@ class EngineModel:
     def decode(self, n_steps):
         """Greedy decoding: each step feeds the previous step's argmax; asynchronous."""
         self.dev._check(self._fn("decode")(self._h, None, n_steps))
+
+    def _per_row(self, x, dtype):
+        """A device slice of one value per sequence: a Slice as it is, a number or an array uploaded."""
+        if x is None or hasattr(x, "_h"):
+            return x
+        x = np.array(np.broadcast_to(np.asarray(x, dtype), (self.batch,)))
+        return self.dev.slice_from_values(x)
+
+    def sample(self, u, temperature=None, top_k=None, top_p=None, min_p=None, prob=None):
+        """Chooses the tokens of the last logits from the random numbers ``u`` (0 <= u < 1) instead of greedily: the next
+        ``decode(1)`` feeds them and :meth:`next_tokens` reads them.  Every argument is one number for all sequences, an array of one
+        per sequence or a device Slice; ``prob``, a Slice, takes the tokens' probabilities.  Asynchronous; a value outside its
+        range is raised by the device's next ``synchronize``."""
+        rows = [self._per_row(x, d) for x, d in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32), (u, np.float32))]
+        self.dev._check(self._fn("sample")(self._h, *[r._h if r is not None else None for r in rows], prob._h if prob is not None else None))
 
     def logits(self):
         """f32 [batch, vocab]; a tensor-parallel rank returns its columns
