@@ -5,7 +5,10 @@
 // by index, at which the running sum of what stays exceeds u times its total.
 //
 // A row is held in the shared memory of one cluster of up to 8 CTAs: it is read from memory once.  Every cut is a threshold on the
-// logit (and, among equal ones, on the index), found by radix selection over the logits' bits, 8 at a time, without a sort.
+// logit (and, among equal ones, on the index).  It is found without a sort: a histogram over the distance from the best logit, in
+// steps of T / 32, says in which step the cut falls; the tokens up to that step, where they are few, are gathered and ranked against
+// one another, and the whole choice is made among them; where they are many only those of that step are ranked; where these are many too
+// (equal logits, a flat row), the next histogram divides the step by the logits' bits, until one logit or few tokens are left.
 //
 // Weights are summed as integers, in units of 2^-44 of the largest one: sums do not depend on their order, so that any number of CTAs and
 // any order of atomics gives the same token, and 2^18 tokens fit 63 bits.  A choice between neighbours hangs on sums that differ
@@ -26,7 +29,9 @@ using ugb_tc::mapa_u32;
 using ugb_tc::smem_u32;
 typedef unsigned long long u64;
 
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 256, COPIES = 4, CLUSTER_MAX = 8;
+constexpr int THREADS = 512, WARPS = THREADS / 32, CLUSTER_MAX = 8;
+constexpr int STEPS = 1024, RANKED = 256;
+constexpr float STEPS_PER_T = 32.0f;                       // 1024 steps reach to exp(-32) < 2^-45: what is beyond weighs nothing
 constexpr double UNIT = 17592186044416.0;                  // 2^44
 
 struct Params {
@@ -44,6 +49,7 @@ __device__ __forceinline__ uint32_t key_of(float x) {      // ascending with the
   const uint32_t b = __float_as_uint(x + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 __device__ __forceinline__ u64 peer_u64(uint32_t addr, int rank) {
   u64 v;
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(mapa_u32(addr, (uint32_t)rank)) : "memory");
@@ -52,17 +58,38 @@ __device__ __forceinline__ u64 peer_u64(uint32_t addr, int rank) {
 
 struct Shared {
   u64 warp_sum[WARPS];
-  u64 total[2][BINS];                                      // by digit, of this CTA
-  uint32_t lo[2][BINS * COPIES], hi[2][BINS * COPIES];
-  u64 slot[16];                                            // what the peers read: one slot per exchange, none is written twice
+  double power[64];                                        // 2^(i / 64)
+  u64 hist[STEPS];
+  u64 in_step[RANKED], before_step[RANKED];                // tokens by place()
+  u64 ranked[RANKED], sorted[RANKED];
+  int count[THREADS];
+  int n_in, n_before;
+  uint32_t key_min, key_max;                               // of the step's tokens
+  u64 slot[16];                                            // what the peers read: none is written twice without a cluster barrier behind the reads
   u64 pick[4];
 };
 
+// Weights by Tang's table method for the exponential: e^y = 2^(n / 64) e^r, |r| <= ln 2 / 128, e^r by its series to r^4 (4e-14).
 struct Weights {
   float best;
   double inv_t;
-  __device__ __forceinline__ double exact(float x) const { return x == best ? 1.0 : exp(((double)x - (double)best) * inv_t); }
-  __device__ __forceinline__ u64 units(float x) const { return (u64)__double2ll_rn(exact(x) * UNIT); }
+  const double *power;
+  __device__ __forceinline__ double exact(float x) const {
+    if (x == best) return 1.0;
+    const double y = ((double)x - (double)best) * inv_t;
+    if (!(y > -40.0)) return 0.0;                          // below half a unit
+    const double shifted = fma(y, 92.332482616893656877, 6755399441055744.0);   // 64 / ln 2; + 1.5 * 2^52: the integer is in the low bits
+    const int n = __double2loint(shifted);
+    const double r = fma(shifted - 6755399441055744.0, -0.010830424696249145, y);
+    double e = fma(r, 1.0 / 24.0, 1.0 / 6.0);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0) * power[n & 63];
+    return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
+  }
+  // in units of 2^-44: the low bits of the sum with 2^8, whose last place that is
+  __device__ __forceinline__ u64 of(double w) const { return (u64)(__double_as_longlong(w + 256.0) - __double_as_longlong(256.0)); }
+  __device__ __forceinline__ u64 units(float x) const { return of(exact(x)); }
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -82,90 +109,50 @@ __device__ __forceinline__ u64 block_sum(u64 v, Shared &sh) {
   return v;
 }
 
-// The logits of one row that this cluster holds, and where a CTA stands in it.
-struct Row {
-  const float *x;
+// Order of a token: falling logit, then rising index.  A larger place comes first.
+__device__ __forceinline__ u64 place(uint32_t key, int index) { return ((u64)key << 32) | (uint32_t)~(uint32_t)index; }
+__device__ __forceinline__ uint32_t key_at(u64 place) { return (uint32_t)(place >> 32); }
+__device__ __forceinline__ int index_at(u64 place) { return (int)~(uint32_t)place; }
+
+// The logits of one row that this CTA holds, and where it stands in the cluster.
+template <typename T> struct Row {
+  const T *x;
   int base, len, rank, size, seg;
-  __device__ __forceinline__ int from() const { return min(len, (int)threadIdx.x * seg); }
-  __device__ __forceinline__ int to() const { return min(len, ((int)threadIdx.x + 1) * seg); }
+  __device__ __forceinline__ float at(int i) const { return (float)x[i]; }
+  // f(index in the CTA, logit) for this thread's share, four loads ahead
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+    const int from = min(len, (int)threadIdx.x * seg), to = min(len, ((int)threadIdx.x + 1) * seg);
+    int i = from;
+    for (; i + 4 <= to; i += 4) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = at(i + j);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(i + j, v[j]);
+    }
+    for (; i < to; ++i) f(i, at(i));
+  }
 };
 
 // Sum over the cluster of what the CTAs put in; `before`: that of lower ranks.
-__device__ __forceinline__ u64 cluster_sum(u64 mine, const Row &r, Shared &sh, int slot, u64 *before = nullptr) {
+template <typename T> __device__ __forceinline__ u64 cluster_sum(u64 mine, const Row<T> &r, Shared &sh, int slot, u64 *before) {
   if (threadIdx.x == 0) sh.slot[slot] = mine;
   cluster_sync_all();
-  u64 all = 0, low = 0;
-  for (int c = 0; c < r.size; ++c) {
-    const u64 v = peer_u64(smem_u32(&sh.slot[slot]), c);
-    if (c < r.rank) low += v;
-    all += v;
+  u64 v[CLUSTER_MAX], all = 0, low = 0;
+#pragma unroll
+  for (int c = 0; c < CLUSTER_MAX; ++c) v[c] = c < r.size ? peer_u64(smem_u32(&sh.slot[slot]), c) : 0;
+#pragma unroll
+  for (int c = 0; c < CLUSTER_MAX; ++c) {
+    if (c < r.rank) low += v[c];
+    all += v[c];
   }
-  if (before) *before = low;
+  *before = low;
   return all;
 }
 
-// The largest key at which the running sum over falling keys reaches `target` (>= 1, at most the whole sum): its key, and the sum above it.
-template <typename F>
-__device__ void select_key(const Row &r, Shared &sh, u64 target, F weigh, uint32_t *key, u64 *above) {
-  uint32_t prefix = 0;
-  u64 over = 0;
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass, par = pass & 1;
-    __syncthreads();                                       // the same buffers' last readers, two passes ago, passed a cluster barrier since
-    for (int i = threadIdx.x; i < BINS * COPIES; i += THREADS) sh.lo[par][i] = sh.hi[par][i] = 0;
-    __syncthreads();
-    for (int i = r.from(); i < r.to(); ++i) {
-      const uint32_t k = key_of(r.x[i]);
-      if (pass > 0 && (k >> (shift + 8)) != prefix) continue;
-      const u64 w = weigh(r.x[i], k);
-      if (w == 0) continue;
-      const int at = ((k >> shift) & 255u) * COPIES + (threadIdx.x & (COPIES - 1));
-      const uint32_t old = atomicAdd(&sh.lo[par][at], (uint32_t)w);
-      const uint32_t high = (uint32_t)(w >> 32) + (old + (uint32_t)w < old ? 1u : 0u);
-      if (high) atomicAdd(&sh.hi[par][at], high);
-    }
-    __syncthreads();
-    if (threadIdx.x < BINS) {
-      u64 v = 0;
-#pragma unroll
-      for (int c = 0; c < COPIES; ++c) v += ((u64)sh.hi[par][threadIdx.x * COPIES + c] << 32) + sh.lo[par][threadIdx.x * COPIES + c];
-      sh.total[par][threadIdx.x] = v;
-    }
-    cluster_sync_all();
-    // every warp adds up all bins by itself: lane l those of digits 255 - 8 l downwards
-    u64 v[8], mine = 0;
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = 0;
-      for (int c = 0; c < r.size; ++c) v[j] += peer_u64(smem_u32(&sh.total[par][255 - 8 * lane - j]), c);
-      mine += v[j];
-    }
-    u64 run = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 n = __shfl_up_sync(0xffffffffu, run, o);
-      if (lane >= o) run += n;
-    }
-    const int owner = __ffs(__ballot_sync(0xffffffffu, over + run >= target)) - 1;
-    u64 sum = over + run - mine;                           // of the digits above this lane's
-    int digit = 0;
-    bool found = false;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (!found && sum + v[j] >= target) { found = true; digit = 255 - 8 * lane - j; }
-      if (!found) sum += v[j];
-    }
-    over = __shfl_sync(0xffffffffu, sum, owner & 31);
-    prefix = (prefix << 8) | (uint32_t)__shfl_sync(0xffffffffu, digit, owner & 31);
-  }
-  *key = prefix;
-  *above = over;
-}
-
 // The first index, over the whole row, at which the running sum of the weights exceeds `target`; in every CTA.  `mine`: this thread's sum.
-template <typename F>
-__device__ int find_index(const Row &r, Shared &sh, u64 target, u64 mine, u64 before, F weigh, int slot, u64 *weight = nullptr) {
+template <typename T, typename F>
+__device__ int find_index(const Row<T> &r, Shared &sh, u64 target, u64 mine, u64 before, F weigh, int slot, u64 *weight) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   u64 run = mine;
 #pragma unroll
@@ -181,17 +168,17 @@ __device__ int find_index(const Row &r, Shared &sh, u64 target, u64 mine, u64 be
   for (int w = 0; w < warp; ++w) low += sh.warp_sum[w];
   if (low + run - mine <= target && target < low + run) {  // one thread of one CTA
     u64 sum = low + run - mine;
-    for (int i = r.from(); i < r.to(); ++i) {
-      const u64 w = weigh(r.x[i], r.base + i);
+    bool open = true;
+    r.each([&](int i, float v) {
+      const u64 w = weigh(v, r.base + i);
       sum += w;
-      if (sum > target) {
+      if (open && sum > target) {
+        open = false;
         sh.slot[slot] = (u64)(r.base + i) + 1;
         sh.slot[slot + 1] = w;
-        break;
       }
-    }
+    });
   }
-  __syncthreads();
   cluster_sync_all();
   u64 at = 0, w = 0;
   for (int c = 0; c < r.size; ++c) {
@@ -202,25 +189,201 @@ __device__ int find_index(const Row &r, Shared &sh, u64 target, u64 mine, u64 be
   return (int)at - 1;
 }
 
-template <typename T> __device__ __forceinline__ float load1(const T *p) { return (float)*p; }
+// Into which of STEPS steps a token falls, by falling logit; STEPS: beyond all, -1: before all.
+struct ByDistance {                                        // from the best logit; rounding keeps the order
+  float best, per_unit;
+  __device__ __forceinline__ int of(float x) const {
+    const float d = x == best ? 0.0f : (best - x) * per_unit;
+    return d < (float)STEPS ? (int)d : STEPS;
+  }
+};
+struct ByKey {                                             // of the keys min .. max
+  uint32_t min, max;
+  int shift;
+  __device__ __forceinline__ int of(float x) const {
+    const uint32_t k = key_of(x);
+    return k > max ? -1 : k < min ? STEPS : (int)((max - k) >> shift);
+  }
+};
+
+// Adds weigh(logit, index) of the tokens of all steps to the histogram, over the cluster, and finds the step in which the running sum reaches the
+// target that `goal` makes of the whole sum.  Returns the step (STEPS: it is not reached); above: the sum before it, within: its own.
+template <typename T, typename S, typename F, typename G>
+__device__ int find_step(const Row<T> &r, Shared &sh, const S &steps, F weigh, G goal, u64 *above, u64 *within, u64 *whole, u64 *target) {
+  for (int i = threadIdx.x; i < STEPS; i += THREADS) sh.hist[i] = 0;
+  if (threadIdx.x == 0) {
+    sh.n_in = sh.n_before = 0;
+    sh.key_min = 0xffffffffu;
+    sh.key_max = 0;
+  }
+  __syncthreads();
+  r.each([&](int i, float v) {
+    const int at = steps.of(v);
+    const u64 w = at < 0 || at >= STEPS ? 0 : weigh(v, r.base + i);
+    if (w) {
+      uint32_t *h = reinterpret_cast<uint32_t *>(&sh.hist[at]);        // 64 bits in two halves: shared memory adds 32 at a time
+      const uint32_t old = atomicAdd(h, (uint32_t)w);
+      const uint32_t high = (uint32_t)(w >> 32) + (old + (uint32_t)w < old ? 1u : 0u);
+      if (high) atomicAdd(h + 1, high);
+    }
+  });
+  cluster_sync_all();
+  constexpr int PER = STEPS / THREADS;
+  u64 v[PER], mine = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    u64 c[CLUSTER_MAX];
+#pragma unroll
+    for (int k = 0; k < CLUSTER_MAX; ++k) c[k] = k < r.size ? peer_u64(smem_u32(&sh.hist[threadIdx.x * PER + j]), k) : 0;
+    v[j] = 0;
+#pragma unroll
+    for (int k = 0; k < CLUSTER_MAX; ++k) v[j] += c[k];
+    mine += v[j];
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 run = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 n = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += n;
+  }
+  if (lane == 31) sh.warp_sum[warp] = run;
+  if (threadIdx.x == 0) sh.pick[0] = STEPS;
+  __syncthreads();
+  u64 all = 0, low = run - mine;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) low += sh.warp_sum[w];
+    all += sh.warp_sum[w];
+  }
+  *whole = all;
+  const u64 t = goal(all);
+  *target = t;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (low < t && t <= low + v[j]) {
+      sh.pick[0] = (u64)(threadIdx.x * PER + j);
+      sh.pick[1] = low;
+      sh.pick[2] = v[j];
+    }
+    low += v[j];
+  }
+  __syncthreads();
+  *above = sh.pick[1];
+  *within = sh.pick[2];
+  return (int)sh.pick[0];
+}
+
+// Lists the tokens of step `in` and (before) of the steps before it, up to RANKED of each kind, every CTA its own.  n_in, n_before: how many there
+// are in the cluster (more than RANKED: that many or more); min, max: the keys of those in the step.
+template <typename T, typename S, typename F>
+__device__ void gather(const Row<T> &r, Shared &sh, const S &steps, int in, bool before, F valid, int slot, int *n_in, int *n_before, uint32_t *min_key, uint32_t *max_key) {
+  uint32_t lo = 0xffffffffu, hi = 0;
+  r.each([&](int i, float x) {
+    const int at = steps.of(x);
+    if (at < 0 || at > in || at == STEPS || (at < in && !before) || !valid(x, r.base + i)) return;
+    const uint32_t k = key_of(x);
+    if (at == in) { lo = min(lo, k); hi = max(hi, k); }
+    int *n = at == in ? &sh.n_in : &sh.n_before;
+    if (*reinterpret_cast<volatile int *>(n) > RANKED) return;
+    const int j = atomicAdd(n, 1);
+    if (j < RANKED) (at == in ? sh.in_step : sh.before_step)[j] = place(k, r.base + i);
+  });
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if ((threadIdx.x & 31) == 0) {
+    atomicMin(&sh.key_min, lo);
+    atomicMax(&sh.key_max, hi);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    sh.slot[slot] = ((u64)(uint32_t)sh.n_before << 32) | (uint32_t)sh.n_in;
+    sh.slot[slot + 1] = ((u64)sh.key_max << 32) | sh.key_min;
+  }
+  cluster_sync_all();
+  *n_in = *n_before = 0;
+  lo = 0xffffffffu;
+  hi = 0;
+  for (int c = 0; c < r.size; ++c) {
+    const u64 v = peer_u64(smem_u32(&sh.slot[slot]), c), k = peer_u64(smem_u32(&sh.slot[slot + 1]), c);
+    *n_in += (int)(uint32_t)v;
+    *n_before += (int)(v >> 32);
+    lo = min(lo, (uint32_t)k);
+    hi = max(hi, (uint32_t)(k >> 32));
+  }
+  *min_key = lo;
+  *max_key = hi;
+}
+
+// Copies the peers' lists (both, or those of the step alone) together.  At most RANKED tokens, the caller has seen to that.
+template <typename T> __device__ void collect(const Row<T> &r, Shared &sh, int slot, bool both) {
+  int at = 0;
+  for (int c = 0; c < r.size; ++c) {
+    const u64 v = peer_u64(smem_u32(&sh.slot[slot]), c);
+    const int n_in = (int)(uint32_t)v, n = n_in + (both ? (int)(v >> 32) : 0);
+    if ((int)threadIdx.x < n) sh.ranked[at + threadIdx.x] = peer_u64(smem_u32((int)threadIdx.x < n_in ? &sh.in_step[threadIdx.x] : &sh.before_step[threadIdx.x - n_in]), c);
+    at += n;
+  }
+  __syncthreads();
+}
+
+// sh.ranked[0 .. n) -> sh.sorted, the largest first.  THREADS / RANKED threads count what is ahead of a value.
+__device__ __forceinline__ void sort_ranked(Shared &sh, int n) {
+  const int i = threadIdx.x & (RANKED - 1);
+  const u64 me = i < n ? sh.ranked[i] : 0;
+  int ahead = 0;
+  if (i < n) {
+#pragma unroll 4
+    for (int j = threadIdx.x / RANKED; j < n; j += THREADS / RANKED) ahead += sh.ranked[j] > me ? 1 : 0;
+  }
+  sh.count[threadIdx.x] = ahead;
+  __syncthreads();
+  if ((int)threadIdx.x < n) {
+#pragma unroll
+    for (int k = 1; k < THREADS / RANKED; ++k) ahead += sh.count[threadIdx.x + k * RANKED];
+    sh.sorted[ahead] = me;
+  }
+  __syncthreads();
+}
+
+// Sum of the values of the threads before this one.
+__device__ __forceinline__ u64 block_before(u64 v, Shared &sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 run = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 n = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += n;
+  }
+  __syncthreads();
+  if (lane == 31) sh.warp_sum[warp] = run;
+  __syncthreads();
+  u64 low = run - v;
+  for (int w = 0; w < warp; ++w) low += sh.warp_sum[w];
+  return low;
+}
+
+__device__ __forceinline__ float load1(const float *p) { return *p; }
+__device__ __forceinline__ float load1(const __nv_bfloat16 *p) { return (float)*p; }
 
 // grid (cluster size x rows): one cluster per row.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 sample_kernel(Params p, int size) {
-  extern __shared__ __align__(16) float x[];
+  extern __shared__ __align__(16) unsigned char held[];
+  T *x = reinterpret_cast<T *>(held);
   __shared__ Shared sh;
-  const int row = blockIdx.x / size, rank = blockIdx.x % size;
-  Row r;
-  r.x = x; r.rank = rank; r.size = size; r.seg = p.seg;
-  r.base = min(p.vocab, rank * p.chunk);
+  const int row = blockIdx.x / size, me = blockIdx.x % size;
+  Row<T> r;
+  r.x = x; r.rank = me; r.size = size; r.seg = p.seg;
+  r.base = min(p.vocab, me * p.chunk);
   r.len = min(p.vocab - r.base, p.chunk);
   const float temperature = p.temperature ? p.temperature[row] : 1.0f, top_p = p.top_p ? p.top_p[row] : 1.0f, min_p = p.min_p ? p.min_p[row] : 0.0f;
   const float u = p.u[row];
   const int top_k = p.top_k ? p.top_k[row] : 0;
   // negated comparisons: a NaN is refused
   if (!(temperature >= 0.0f) || isinf(temperature) || top_k < 0 || !(top_p > 0.0f) || !(min_p >= 0.0f && min_p <= 1.0f) || !(u >= 0.0f && u < 1.0f)) {
-    if (rank == 0 && threadIdx.x == 0 && atomicCAS(&p.status->code, 0u, (unsigned)UGB_ERR_INVALID) == 0u) p.status->detail = (unsigned)row;
+    if (me == 0 && threadIdx.x == 0 && atomicCAS(&p.status->code, 0u, (unsigned)UGB_ERR_INVALID) == 0u) p.status->detail = (unsigned)row;
     return;                                                // the whole cluster: the row is left as it was
   }
   const T *g = (const T *)p.logits + (long long)row * p.ld + r.base;
@@ -228,7 +391,7 @@ sample_kernel(Params p, int size) {
   int at = 0x7fffffff;
   auto take = [&](float v, int i) {
     v = v != v ? -INFINITY : v;                            // a NaN is no candidate
-    x[i] = v;
+    x[i] = (T)v;
     if (v > best || (v == best && i < at)) { best = v; at = i; }
   };
   constexpr int PER = 16 / (int)sizeof(T);
@@ -249,8 +412,8 @@ sample_kernel(Params p, int size) {
   } else {
     for (int i = threadIdx.x; i < r.len; i += THREADS) take(load1(g + i), i);
   }
-  // the best logit, equal ones by index: the largest (key, ~index)
-  u64 top = at == 0x7fffffff ? 0 : ((u64)key_of(best) << 32) | (uint32_t)~(uint32_t)(r.base + at);
+  if (threadIdx.x < 64) sh.power[threadIdx.x] = exp2(threadIdx.x / 64.0);
+  u64 top = at == 0x7fffffff ? 0 : place(key_of(best), r.base + at);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   if ((threadIdx.x & 31) == 0) sh.warp_sum[threadIdx.x >> 5] = top;
@@ -261,69 +424,116 @@ sample_kernel(Params p, int size) {
   }
   cluster_sync_all();
   top = 0;
-  for (int c = 0; c < size; ++c) top = max(top, peer_u64(smem_u32(&sh.slot[0]), c));
-  const uint32_t top_key = (uint32_t)(top >> 32);
-  const int top_index = (int)~(uint32_t)top;
+#pragma unroll
+  for (int c = 0; c < CLUSTER_MAX; ++c)
+    if (c < size) top = max(top, peer_u64(smem_u32(&sh.slot[0]), c));
   Weights weights;
-  weights.best = __uint_as_float(top_key & 0x80000000u ? top_key & 0x7fffffffu : ~top_key);
+  weights.best = value_of(key_at(top));
   weights.inv_t = 1.0 / (double)temperature;
-  int token = top_index;
+  weights.power = sh.power;
+  int token = index_at(top);
   float prob = 1.0f;
   if (weights.best == -INFINITY) {                         // nothing to choose from
     token = -1;
     prob = 0.0f;
   } else if (temperature > 0.0f) {
-    uint32_t cut = 0;                                      // keys above `cut` stay, and of those at it the ones of index <= `last`
-    u64 ties = 0;                                          // how many of those at it, 0: all
-    if (top_k > 0 && top_k < p.vocab) {
-      u64 above;
-      select_key(r, sh, (u64)top_k, [](float, uint32_t) { return (u64)1; }, &cut, &above);
-      ties = (u64)top_k - above;
-    }
-    if (top_p < 1.0f) {
-      u64 sum = 0, at_cut = 0;
-      for (int i = r.from(); i < r.to(); ++i) {
-        const uint32_t k = key_of(x[i]);
-        if (k > cut || (ties == 0 && k == cut)) sum += weights.units(x[i]);
-      }
-      sum = cluster_sum(block_sum(sum, sh), r, sh, 1);
-      if (ties) {                                          // equal logits weigh the same
-        const float c = __uint_as_float(cut & 0x80000000u ? cut & 0x7fffffffu : ~cut);
-        at_cut = weights.units(c);
-        sum += ties * at_cut;
-      }
-      const u64 target = min(sum, max((u64)1, (u64)ceil((double)top_p * (double)sum)));
-      u64 above;
-      uint32_t k1;
-      const uint32_t k0 = cut;
-      select_key(r, sh, target, [&](float v, uint32_t k) { return k >= k0 ? weights.units(v) : (u64)0; }, &k1, &above);
-      cut = k1;
-      const u64 w = weights.units(__uint_as_float(cut & 0x80000000u ? cut & 0x7fffffffu : ~cut));
-      ties = (target - above + w - 1) / w;
-    }
-    int last = p.vocab;
-    if (ties) {
-      u64 mine = 0, before;
-      for (int i = r.from(); i < r.to(); ++i) mine += key_of(x[i]) == cut ? 1 : 0;
-      const u64 all = cluster_sum(block_sum(mine, sh), r, sh, 2, &before);
-      if (ties < all) last = find_index(r, sh, ties - 1, mine, before, [&](float v, int) { return (u64)(key_of(v) == cut ? 1 : 0); }, 4);
-    }
     const double low = (double)min_p;
-    auto kept = [&](float v, int i) -> u64 {
-      const uint32_t k = key_of(v);
-      if (k < cut || (k == cut && i > last)) return 0;
-      const double w = weights.exact(v);
-      return w >= low ? (u64)__double2ll_rn(w * UNIT) : 0;
+    auto share_of = [&](u64 sum) { return min(sum, max((u64)1, (u64)ceil((double)top_p * (double)sum))); };
+    auto drawn = [&](u64 sum) { return min(sum - 1, __umul64hi((u64)((double)u * 18446744073709551616.0), sum)); };
+    const bool by_k = top_k > 0 && top_k < p.vocab, by_p = top_p < 1.0f;
+    // behind this step everything weighs less than min_p (a step more, for the rounding of both sides)
+    const int low_step = min_p > 0.0f ? min(STEPS - 1, (int)(-logf(min_p) * STEPS_PER_T) + 1) : STEPS - 1;
+    u64 cut = 0;                                           // tokens of this place and the ones before it stay
+    auto stays = [&](float v, int i) { return place(key_of(v), i) >= cut; };
+    // The choice among n ranked tokens, all that can be chosen; sum: what top_p is a share of, unless that is the first top_k.  CTA 0 alone.
+    auto finish = [&](int n, bool first_k, u64 sum) {
+      sort_ranked(sh, n);
+      const u64 e = (int)threadIdx.x < n ? sh.sorted[threadIdx.x] : 0;
+      const double w = (int)threadIdx.x < n ? weights.exact(value_of(key_at(e))) : 0.0;
+      bool in = (int)threadIdx.x < n && (!first_k || (int)threadIdx.x < top_k);
+      u64 units = in ? weights.of(w) : 0;
+      if (by_p) {
+        if (first_k) sum = block_sum(units, sh);
+        const u64 before = block_before(units, sh);        // a barrier: by every thread, whatever `in` is
+        in = in && before < share_of(sum);
+      }
+      in = in && w >= low;
+      // what stays is a beginning: its tokens by index, the lowest first
+      const int m = __syncthreads_count(in);
+      if (in) sh.ranked[threadIdx.x] = ((u64)(uint32_t)~(uint32_t)index_at(e) << 32) | key_at(e);
+      __syncthreads();
+      sort_ranked(sh, m);
+      const u64 f = (int)threadIdx.x < m ? sh.sorted[threadIdx.x] : 0;
+      units = (int)threadIdx.x < m ? weights.units(value_of((uint32_t)f)) : 0;
+      const u64 all = block_sum(units, sh), before = block_before(units, sh), target = drawn(all);
+      if (before <= target && target < before + units) {
+        p.tokens[row] = (int)~(uint32_t)(f >> 32);
+        if (p.prob) p.prob[row] = (float)((double)units / (double)all);
+      }
     };
-    u64 mine = 0, before;
-    for (int i = r.from(); i < r.to(); ++i) mine += kept(x[i], r.base + i);
-    const u64 all = cluster_sum(block_sum(mine, sh), r, sh, 3, &before);
-    const u64 target = min(all - 1, __umul64hi((u64)((double)u * 18446744073709551616.0), all));
-    u64 w;
-    token = find_index(r, sh, target, mine, before, kept, 6, &w);
+    bool done = false;
+    // Finds the cut at which the running sum of weigh over the tokens that stay reaches a target, or makes the choice.
+    auto narrow = [&](auto weigh, auto goal, bool first_k, int slot) {
+      ByDistance steps{weights.best, STEPS_PER_T / temperature};
+      u64 above, within, whole, target;
+      int n_in, n_before;
+      uint32_t key_min, key_max;
+      const int step = find_step(r, sh, steps, weigh, goal, &above, &within, &whole, &target);
+      const bool beyond = step == STEPS;                   // fewer tokens weigh anything than top_k: all of them stay
+      const int in = min(beyond ? STEPS - 1 : step, by_p && first_k ? STEPS - 1 : low_step);   // top_p after top_k needs all the first top_k
+      gather(r, sh, steps, in, true, stays, slot, &n_in, &n_before, &key_min, &key_max);
+      if (n_in + n_before <= RANKED) {
+        if (me == 0) collect(r, sh, slot, true);
+        cluster_sync_all();                                // the others leave
+        if (me == 0) finish(n_in + n_before, first_k, whole);
+        done = true;
+        return;
+      }
+      if (beyond || in < step) return;                     // this cut takes away nothing that the next ones or min_p leave
+      for (;;) {
+        if (n_in <= RANKED) {
+          collect(r, sh, slot, false);
+          sort_ranked(sh, n_in);
+          const u64 e = (int)threadIdx.x < n_in ? sh.sorted[threadIdx.x] : 0;
+          const u64 w = (int)threadIdx.x < n_in ? weigh(value_of(key_at(e)), index_at(e)) : 0, sum = above + block_before(w, sh);
+          if (sum < target && target <= sum + w) sh.pick[3] = e;
+          __syncthreads();
+          cut = sh.pick[3];
+          break;
+        }
+        if (key_min == key_max) {                          // equal logits, which weigh the same: by index
+          const u64 w = first_k ? 1 : weights.units(value_of(key_min)), ties = (target - above + w - 1) / w;
+          auto tied = [&](float v, int i) { return (u64)(key_of(v) == key_min && stays(v, i) ? 1 : 0); };
+          u64 mine = 0, before;
+          r.each([&](int i, float v) { mine += tied(v, r.base + i); });
+          cluster_sum(block_sum(mine, sh), r, sh, slot + 2, &before);
+          const int last = find_index(r, sh, ties - 1, mine, before, tied, slot + 3, nullptr);
+          cut = place(key_min, last);
+          break;
+        }
+        ByKey keys{key_min, key_max, max(0, 22 - __clz(key_max - key_min))};     // (max - min) >> shift < 1024
+        const u64 over = above;
+        const int at = find_step(r, sh, keys, weigh, [&](u64) { return target - over; }, &above, &within, &whole, &target);
+        above += over;
+        target += over;
+        gather(r, sh, keys, at, false, stays, slot, &n_in, &n_before, &key_min, &key_max);
+      }
+      __syncthreads();
+    };
+    if (by_k) narrow([&](float, int) { return (u64)1; }, [&](u64) { return (u64)top_k; }, true, 1);
+    if (!done && by_p) narrow([&](float v, int i) { return stays(v, i) ? weights.units(v) : (u64)0; }, share_of, false, 6);
+    if (done) return;
+    auto kept = [&](float v, int i) -> u64 {
+      const double w = weights.exact(v);
+      return stays(v, i) && w >= low ? weights.of(w) : 0;
+    };
+    u64 mine = 0, before, w;
+    r.each([&](int i, float v) { mine += kept(v, r.base + i); });
+    const u64 all = cluster_sum(block_sum(mine, sh), r, sh, 11, &before);
+    token = find_index(r, sh, drawn(all), mine, before, kept, 12, &w);
     prob = (float)((double)w / (double)all);
   }
-  if (rank == 0 && threadIdx.x == 0) {
+  if (me == 0 && threadIdx.x == 0) {
     p.tokens[row] = token;
     if (p.prob) p.prob[row] = prob;
   }
@@ -334,10 +544,10 @@ template <typename T>
 int32_t launch(ugb_device *dev, const Params &p, int size) {
   static bool attr_set[64] = {};
   if (!attr_set[dev->ordinal & 63]) {
-    UGB_CUDA(dev, cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, UGB_SAMPLE_VOCAB_MAX / CLUSTER_MAX * 4));
+    UGB_CUDA(dev, cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, UGB_SAMPLE_VOCAB_MAX / CLUSTER_MAX * (int)sizeof(T)));
     attr_set[dev->ordinal & 63] = true;
   }
-  const cudaError_t e = ugb_launch_cluster(sample_kernel<T>, dim3((unsigned)(p.rows * size)), dim3(THREADS), (size_t)p.chunk * 4, dev->stream, false, size, p, size);
+  const cudaError_t e = ugb_launch_cluster(sample_kernel<T>, dim3((unsigned)(p.rows * size)), dim3(THREADS), (size_t)p.chunk * sizeof(T), dev->stream, false, size, p, size);
   if (e != cudaSuccess) return ugb_fail(dev, UGB_ERR_CUDA, "launch of sample_kernel failed: %s", cudaGetErrorString(e));
   return ugb_after_launch(dev, "sample_kernel");
 }
