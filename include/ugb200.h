@@ -759,12 +759,27 @@ UGB_API int32_t ugb_tree_inputs(ugb_device *dev, const ugb_slice *pre, const ugb
                                 const ugb_slice *pos, const ugb_slice *parents, ugb_slice *q, ugb_slice *kcache, ugb_slice *vcache,
                                 size_t b, size_t t, size_t heads, size_t kv_heads, size_t dim, size_t vdim, size_t rot_dims,
                                 int32_t interleaved, int32_t qk_norm, float eps, size_t t_max);
+/* Attention of t drafted nodes: query i attends the pos[s] committed positions, its node's ancestors and itself, whose keys and
+ * values are in the cache rows above.  q T [b, t, heads, dq], k, v T [b, kv_heads, t_max, dq / dv], out T [b, t, heads, dv] times
+ * out_scale; query head h reads head h / (heads / kv_heads); dq and dv multiples of 8 up to 256.  Cache rows behind the last node
+ * may hold anything. */
+UGB_API int32_t ugb_tree_attend(ugb_device *dev, const ugb_slice *q, const ugb_slice *k, const ugb_slice *v, const ugb_slice *pos,
+                                const ugb_slice *parents, ugb_slice *out, size_t b, size_t t, size_t heads, size_t kv_heads,
+                                size_t dq, size_t dv, size_t t_max, float scale, float out_scale);
 /* Moves the rows of accepted nodes up behind the committed ones: row pos[s] + path[s, i] of every head of k and v to row
  * pos[s] + i for i < count[s].  k, v T [b, kv_heads, t_max, dq / dv], path I32 [b, most], count I32 [b], most <= 128; the nodes of
  * a path ascend (as along any way down a tree); every other row stays as it was.  A count above most, a path that does
  * not ascend or leaves the cache: UGB_ERR_INVALID at the next ugb_sync, and the sequence is left as it was. */
 UGB_API int32_t ugb_cache_keep(ugb_device *dev, ugb_slice *k, ugb_slice *v, const ugb_slice *pos, const ugb_slice *path,
                                const ugb_slice *count, size_t b, size_t kv_heads, size_t dq, size_t dv, size_t t_max, size_t most);
+/* Attention of t >= 1 new positions over a sliding window and the first positions: query i, at n = pos[s] + i, attends the
+ * positions j <= n with j > n - window or j < sinks.  pos I32 [b], a position for every sequence, -1 as above; k and v
+ * hold the new positions too (row pos[s] + i), and what no query of the block sees (rows ahead of the window, behind the
+ * block) may hold anything.  q, out and head layouts as in ugb_tree_attend; any window >= 1, sinks >= 0.  Both
+ * take scratch for partial results from the device's stream-ordered pool for the duration of the call. */
+UGB_API int32_t ugb_window_attend(ugb_device *dev, const ugb_slice *q, const ugb_slice *k, const ugb_slice *v, const ugb_slice *pos,
+                                  ugb_slice *out, size_t b, size_t t, size_t heads, size_t kv_heads, size_t dq, size_t dv,
+                                  size_t t_max, size_t sinks, size_t window, float scale, float out_scale);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,363 @@
+// Attention of new positions over a sliding window and the first positions of a cache, or over the cache and their ancestors in a
+// tree (ugb_window_attend, ugb_tree_attend; see masked_attention.cuh).
+//
+//   masked_attention_generic_kernel   f32, and heads that the tensor-core kernel does not take: plain FFMA over tiles of 64 keys
+//   masked_combine_kernel             joins the slices of the keys that ran as separate CTAs
+//
+// One pass over the keys with the running maximum and sum of the softmax, in 32 bits, in powers of two.
+#include "masked_attention.cuh"
+
+#include <cuda_bf16.h>
+
+#include <algorithm>
+
+namespace {
+
+using namespace ugb_masked;
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Params {
+  const void *q, *k, *v;
+  void *out;
+  ugb_mask mask;
+  int heads, kv_heads, share, rows, dq, dv, splits;        // rows: t * share, of a sequence and key / value head
+  float scale, out_scale;                                  // scale: with log2(e)
+  float *part_o;                                           // [splits][b][kv_heads][rows][dv]
+  float2 *part_ml;                                         // (maximum, sum) alike
+  ugb_status_word *status;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Whether sequence s is to be computed; raises the status word where its position or its tree is invalid.  By a whole block, and the parents are in `up`
+// behind it.
+template <bool TREE> __device__ __forceinline__ bool check_sequence(const ugb_mask &m, int s, int pos, int *up, ugb_status_word *status) {
+  bool bad = pos < 0 || pos > m.t_max - m.t;
+  if constexpr (TREE) {
+    for (int j = threadIdx.x; j < m.t; j += blockDim.x) {
+      const int a = m.parents[(size_t)s * m.t + j];
+      up[j] = a;
+      bad |= a < -1 || a >= j;
+    }
+  }
+  bad = __syncthreads_or(bad);
+  if (pos == -1) return false;
+  if (bad && threadIdx.x == 0) raise_invalid(status, s);
+  return !bad;
+}
+
+// ------------------------------------------------------------- generic ------
+// grid (row tiles, key / value heads x sequences, slices), 256 threads as 16 x 16: rows ty * RM + i, keys tx + 16 j, columns 4 tx + 64 c.
+// Shared memory, all f32: queries [16 RM][dq + 4], keys and then values of a tile [64][max(dq, dv) + 4], probabilities [16 RM][64 + 4].
+// The products' operands come from shared memory four columns at a time (rows apart by an odd multiple of 16 bytes: no bank conflicts).
+template <typename T, int RM, int NC, bool TREE>
+__global__ void __launch_bounds__(256)
+masked_attention_generic_kernel(Params p) {
+  constexpr int TR = 16 * RM, PLD = KEYS + 4;
+  extern __shared__ __align__(16) float gsm[];
+  __shared__ int up[TREE ? UGB_TREE_MAX : 1];
+  __shared__ uint32_t bits[TREE ? TR * 4 : 1];             // of a row: which nodes its node sees
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, dq = p.dq, dv = p.dv, ld = max(dq, dv) + 4, qld = dq + 4;
+  float *qs = gsm, *ks = qs + TR * qld, *ps = ks + KEYS * ld;
+  const int s = blockIdx.y / p.kv_heads, kvh = blockIdx.y % p.kv_heads, row0 = blockIdx.x * TR, n_rows = min(TR, p.rows - row0);
+  const int pos = p.mask.pos[s];
+  if (!check_sequence<TREE>(p.mask, s, pos, up, p.status)) return;
+  if constexpr (TREE) {
+    for (int r = threadIdx.x; r < TR; r += 256) {
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (r < n_rows)
+        for (int j = (row0 + r) / p.share; j >= 0; j = up[j]) w[j >> 5] |= 1u << (j & 31);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bits[r * 4 + e] = w[e];
+    }
+  }
+  const T *q = (const T *)p.q, *k = (const T *)p.k + ((size_t)s * p.kv_heads + kvh) * p.mask.t_max * dq, *v = (const T *)p.v + ((size_t)s * p.kv_heads + kvh) * p.mask.t_max * dv;
+  for (int i = threadIdx.x; i < TR * dq; i += 256) {
+    const int r = i / dq, c = i - r * dq, row = row0 + r;
+    qs[r * qld + c] = r < n_rows ? (float)q[(((size_t)s * p.mask.t + row / p.share) * p.heads + kvh * p.share + row % p.share) * dq + c] : 0.f;
+  }
+  const int i0 = row0 / p.share, i1 = (row0 + n_rows - 1) / p.share;
+  const Span span = span_of<TREE>(p.mask, pos, i0, i1);
+  const int per = (span.tiles + p.splits - 1) / p.splits, first = blockIdx.z * per, last = min(span.tiles, first + per);
+  float m[RM], l[RM], o[RM][4 * NC];
+  int at[RM];                                              // absolute position of a row's query
+#pragma unroll
+  for (int i = 0; i < RM; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+    at[i] = pos + (row0 + ty * RM + i) / p.share;
+#pragma unroll
+    for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
+  }
+  for (int tile = first; tile < last; ++tile) {
+    const int key0 = span.key0(tile);
+    auto seen = [&](int key) { return key < span.first || (key >= span.from && key < span.end); };      // by any row: the others may hold anything
+    __syncthreads();
+    for (int i = threadIdx.x; i < KEYS * dq; i += 256) {
+      const int key = i / dq, c = i - key * dq;
+      ks[key * ld + c] = seen(key0 + key) ? (float)k[(size_t)(key0 + key) * dq + c] : 0.f;
+    }
+    __syncthreads();
+    float sc[RM][4];
+#pragma unroll
+    for (int i = 0; i < RM; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
+    for (int c = 0; c < dq; c += 4) {
+      float4 a[RM], b[4];
+#pragma unroll
+      for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4 *>(qs + (ty * RM + i) * qld + c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4 *>(ks + (tx + 16 * j) * ld + c);
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          sc[i][j] = fmaf(a[i].x, b[j].x, sc[i][j]);
+          sc[i][j] = fmaf(a[i].y, b[j].y, sc[i][j]);
+          sc[i][j] = fmaf(a[i].z, b[j].z, sc[i][j]);
+          sc[i][j] = fmaf(a[i].w, b[j].w, sc[i][j]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = key0 + tx + 16 * j;
+        bool on;
+        if constexpr (TREE) {
+          const int node = key - pos;
+          on = node < 0 || (node < p.mask.t && (bits[(ty * RM + i) * 4 + (node >> 5)] >> (node & 31) & 1u));
+        } else {
+          on = key <= at[i] && (key > at[i] - p.mask.window || key < p.mask.sinks);
+        }
+        sc[i][j] = on ? sc[i][j] * p.scale : -INFINITY;
+        mx = fmaxf(mx, sc[i][j]);
+      }
+#pragma unroll
+      for (int e = 8; e > 0; e >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, e));
+      const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn;       // a row may see nothing of this tile
+      const float alpha = exp2f(m[i] - base);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float w = exp2f(sc[i][j] - base);
+        sum += w;
+        ps[(ty * RM + i) * PLD + tx + 16 * j] = w;
+      }
+      l[i] = l[i] * alpha + sum;                           // of this thread's keys; added up behind the last tile
+      m[i] = mn;
+#pragma unroll
+      for (int c = 0; c < 4 * NC; ++c) o[i][c] *= alpha;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < KEYS * dv; i += 256) {
+      const int key = i / dv, c = i - key * dv;
+      ks[key * ld + c] = seen(key0 + key) ? (float)v[(size_t)(key0 + key) * dv + c] : 0.f;
+    }
+    __syncthreads();
+    for (int key = 0; key < KEYS; key += 4) {
+      float4 w[RM];
+#pragma unroll
+      for (int i = 0; i < RM; ++i) w[i] = *reinterpret_cast<const float4 *>(ps + (ty * RM + i) * PLD + key);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          if (4 * tx + 64 * c >= dv) continue;
+          const float4 b = *reinterpret_cast<const float4 *>(ks + (key + e) * ld + 4 * tx + 64 * c);
+#pragma unroll
+          for (int i = 0; i < RM; ++i) {
+            const float a = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+            o[i][4 * c] = fmaf(a, b.x, o[i][4 * c]);
+            o[i][4 * c + 1] = fmaf(a, b.y, o[i][4 * c + 1]);
+            o[i][4 * c + 2] = fmaf(a, b.z, o[i][4 * c + 2]);
+            o[i][4 * c + 3] = fmaf(a, b.w, o[i][4 * c + 3]);
+          }
+        }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < RM; ++i) {
+#pragma unroll
+    for (int e = 8; e > 0; e >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], e);
+    const int r = ty * RM + i, row = row0 + r;
+    if (r >= n_rows) continue;
+    if (p.splits == 1) {
+      const float f = l[i] > 0.f ? p.out_scale / l[i] : 0.f;
+      T *out = (T *)p.out + (((size_t)s * p.mask.t + row / p.share) * p.heads + kvh * p.share + row % p.share) * dv;
+#pragma unroll
+      for (int c = 0; c < 4 * NC; ++c)
+        if (4 * tx + 64 * (c / 4) < dv) out[4 * tx + 64 * (c / 4) + c % 4] = (T)(o[i][c] * f);
+    } else {
+      const size_t slot = ((size_t)blockIdx.z * gridDim.y + blockIdx.y) * p.rows + row;
+      if (tx == 0) p.part_ml[slot] = make_float2(m[i], l[i]);
+#pragma unroll
+      for (int c = 0; c < 4 * NC; ++c)
+        if (4 * tx + 64 * (c / 4) < dv) p.part_o[slot * dv + 4 * tx + 64 * (c / 4) + c % 4] = o[i][c];
+    }
+  }
+}
+
+// ------------------------------------------------------------- combine ------
+// One warp per row: the slices in their order, whatever order they ran in.
+template <typename T, bool TREE>
+__global__ void __launch_bounds__(256)
+masked_combine_kernel(Params p, int pairs) {
+  const size_t n = (size_t)pairs * p.rows, at = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (at >= n) return;
+  const int pair = (int)(at / p.rows), row = (int)(at % p.rows), s = pair / p.kv_heads, kvh = pair % p.kv_heads, pos = p.mask.pos[s];
+  bool bad = pos < 0 || pos > p.mask.t_max - p.mask.t;
+  if constexpr (TREE)
+    for (int j = lane; j < p.mask.t; j += 32) {
+      const int a = p.mask.parents[(size_t)s * p.mask.t + j];
+      bad |= a < -1 || a >= j;
+    }
+  if (__any_sync(0xffffffffu, bad)) return;                // nothing was computed
+  float m = -INFINITY;
+  for (int z = lane; z < p.splits; z += 32) m = fmaxf(m, p.part_ml[(size_t)z * n + at].x);
+#pragma unroll
+  for (int e = 16; e > 0; e >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, e));
+  float l = 0.f;
+  for (int c0 = 0; c0 < p.dv; c0 += 128) {                 // dv is a multiple of 8
+    const int c = c0 + 4 * lane;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    l = 0.f;
+#pragma unroll 4
+    for (int z = 0; z < p.splits; ++z) {
+      const float2 ml = p.part_ml[(size_t)z * n + at];
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+      l = fmaf(f, ml.y, l);
+      if (c < p.dv && f > 0.f) {
+        const float4 v = *reinterpret_cast<const float4 *>(p.part_o + ((size_t)z * n + at) * p.dv + c);
+        acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+      }
+    }
+    const float f = l > 0.f ? p.out_scale / l : 0.f;
+    if (c < p.dv) {
+      T *out = (T *)p.out + (((size_t)s * p.mask.t + row / p.share) * p.heads + kvh * p.share + row % p.share) * p.dv + c;
+      out[0] = (T)(acc.x * f); out[1] = (T)(acc.y * f); out[2] = (T)(acc.z * f); out[3] = (T)(acc.w * f);
+    }
+  }
+}
+
+size_t generic_smem(int dq, int dv, int rows) { return (size_t)(rows * (dq + 4) + KEYS * (std::max(dq, dv) + 4) + rows * (KEYS + 4)) * 4; }
+
+template <typename T, int RM, int NC, bool TREE> cudaError_t launch_generic(dim3 grid, size_t smem, cudaStream_t st, const Params &p) {
+  static bool attr_set[64] = {};
+  int ordinal = 0;
+  cudaError_t e = cudaGetDevice(&ordinal);
+  if (e != cudaSuccess) return e;
+  if (!attr_set[ordinal & 63]) {
+    e = cudaFuncSetAttribute(masked_attention_generic_kernel<T, RM, NC, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)generic_smem(256, 256, 16 * RM));
+    if (e != cudaSuccess) return e;
+    attr_set[ordinal & 63] = true;
+  }
+  masked_attention_generic_kernel<T, RM, NC, TREE><<<grid, 256, smem, st>>>(p);
+  return cudaSuccess;
+}
+template <typename T, int RM, bool TREE> cudaError_t launch_columns(dim3 grid, size_t smem, cudaStream_t st, const Params &p) {
+  if (p.dv <= 64) return launch_generic<T, RM, 1, TREE>(grid, smem, st, p);
+  if (p.dv <= 128) return launch_generic<T, RM, 2, TREE>(grid, smem, st, p);
+  return launch_generic<T, RM, 4, TREE>(grid, smem, st, p);
+}
+template <typename T> cudaError_t launch_rows(bool tree, int rm, dim3 grid, size_t smem, cudaStream_t st, const Params &p) {
+  if (rm == 1) return tree ? launch_columns<T, 1, true>(grid, smem, st, p) : launch_columns<T, 1, false>(grid, smem, st, p);
+  return tree ? launch_columns<T, 4, true>(grid, smem, st, p) : launch_columns<T, 4, false>(grid, smem, st, p);
+}
+
+// Slices of the keys: as many as bring the CTAs to `slots`, of at least two tiles each (a slice costs a round of sums through memory).
+int slices(long long ctas, long long slots, int tiles) {
+  return (int)std::max(1LL, std::min({slots / std::max(1LL, ctas), (long long)(tiles + 1) / 2, 64LL}));
+}
+
+}  // namespace
+
+int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a) {
+  if (a.b == 0 || a.t == 0) return UGB_OK;
+  const bool tree = a.parents != nullptr;
+  Params p;
+  p.q = a.q; p.k = a.k; p.v = a.v; p.out = a.out;
+  p.mask = ugb_mask{a.pos, a.parents, a.t, a.t_max, a.sinks, a.window};
+  p.heads = a.heads; p.kv_heads = a.kv_heads; p.share = a.heads / a.kv_heads; p.rows = a.t * p.share; p.dq = a.dq; p.dv = a.dv;
+  p.scale = a.scale * LOG2E; p.out_scale = a.out_scale; p.part_o = nullptr; p.part_ml = nullptr; p.status = dev->status_dev;
+  // the most keys that a row of tiles can see: the position is on the device
+  const long long reach = tree ? a.t_max : std::min<long long>(a.t_max, (long long)a.window + a.t + a.sinks);
+  const int tiles = (int)((reach + KEYS - 1) / KEYS + 1), pairs = a.b * a.kv_heads;
+  const int rm = p.rows <= 16 ? 1 : 4, row_tiles = (p.rows + 16 * rm - 1) / (16 * rm);
+  const size_t smem = generic_smem(a.dq, a.dv, 16 * rm);
+  p.splits = slices((long long)row_tiles * pairs, 2LL * dev->sm_count, tiles);
+  const size_t n = (size_t)pairs * p.rows;
+  void *work = nullptr;
+  if (p.splits > 1) {
+    UGB_CUDA(dev, ugb_malloc_async(dev, &work, (size_t)p.splits * n * (size_t)(a.dv + 2) * 4));
+    p.part_o = (float *)work;
+    p.part_ml = (float2 *)(p.part_o + (size_t)p.splits * n * a.dv);
+  }
+  const dim3 grid((unsigned)row_tiles, (unsigned)pairs, (unsigned)p.splits);
+  const cudaError_t e = a.f32 ? launch_rows<float>(tree, rm, grid, smem, dev->stream, p) : launch_rows<__nv_bfloat16>(tree, rm, grid, smem, dev->stream, p);
+  int32_t rc = e != cudaSuccess ? ugb_fail(dev, UGB_ERR_CUDA, "launch of masked_attention_generic_kernel failed: %s", cudaGetErrorString(e))
+                                : ugb_after_launch(dev, "masked_attention_generic_kernel");
+  if (rc == UGB_OK && p.splits > 1) {
+    const dim3 rows((unsigned)((n + 7) / 8));
+    if (a.f32) tree ? masked_combine_kernel<float, true><<<rows, 256, 0, dev->stream>>>(p, pairs) : masked_combine_kernel<float, false><<<rows, 256, 0, dev->stream>>>(p, pairs);
+    else tree ? masked_combine_kernel<__nv_bfloat16, true><<<rows, 256, 0, dev->stream>>>(p, pairs) : masked_combine_kernel<__nv_bfloat16, false><<<rows, 256, 0, dev->stream>>>(p, pairs);
+    rc = ugb_after_launch(dev, "masked_combine_kernel");
+  }
+  if (work) cudaFreeAsync(work, dev->stream);
+  return rc;
+}
+
+namespace {
+
+int32_t attend(ugb_device *dev, const char *what, const ugb_slice *q, const ugb_slice *k, const ugb_slice *v, const ugb_slice *pos, const ugb_slice *parents,
+               ugb_slice *out, size_t b, size_t t, size_t heads, size_t kv_heads, size_t dq, size_t dv, size_t t_max, size_t sinks, size_t window, float scale,
+               float out_scale) {
+  UGB_REQUIRE(dev, q && out, UGB_ERR_INVALID, "%s: null slice", what);
+  UGB_REQUIRE(dev, q->dtype == out->dtype && (q->dtype == UGB_BF16 || q->dtype == UGB_F32), UGB_ERR_DTYPE, "%s: activations must be BF16 or F32 alike", what);
+  UGB_REQUIRE(dev, kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && dq % 8 == 0 && dv % 8 == 0 && dq > 0 && dv > 0 && heads <= 65535 && b <= (1u << 20) &&
+                       t_max <= (1u << 30) && t <= t_max && b * kv_heads <= 65535, UGB_ERR_SHAPE, "%s: unsupported shape", what);
+  UGB_REQUIRE(dev, dq <= 256 && dv <= 256, UGB_ERR_UNSUPPORTED, "%s: heads of %zu and %zu values, at most 256", what, dq, dv);
+  UGB_REQUIRE(dev, b * t * heads <= (1u << 30), UGB_ERR_UNSUPPORTED, "%s: %zu positions of %zu sequences in one call", what, t, b);
+  UGB_SLICE(dev, q, q->dtype, b * t * heads * dq);
+  UGB_SLICE(dev, out, q->dtype, b * t * heads * dv);
+  UGB_SLICE(dev, k, q->dtype, b * kv_heads * t_max * dq);
+  UGB_SLICE(dev, v, q->dtype, b * kv_heads * t_max * dv);
+  UGB_SLICE(dev, pos, UGB_I32, b);
+  if (parents) UGB_SLICE(dev, parents, UGB_I32, b * t);
+  UGB_REQUIRE(dev, !ugb_overlap(out, q) && !ugb_overlap(out, k) && !ugb_overlap(out, v), UGB_ERR_INVALID, "%s: in place", what);
+  if (b == 0 || t == 0) return UGB_OK;
+  UGB_CUDA(dev, cudaSetDevice(dev->ordinal));
+  ugb_masked_attention_args a;
+  a.f32 = q->dtype == UGB_F32;
+  a.q = q->ptr; a.k = k->ptr; a.v = v->ptr; a.out = out->ptr; a.pos = (const int *)pos->ptr; a.parents = parents ? (const int *)parents->ptr : nullptr;
+  a.b = (int)b; a.t = (int)t; a.heads = (int)heads; a.kv_heads = (int)kv_heads; a.dq = (int)dq; a.dv = (int)dv; a.t_max = (int)t_max;
+  a.sinks = (int)std::min<size_t>(sinks, t_max); a.window = (int)std::min<size_t>(window, t_max); a.scale = scale; a.out_scale = out_scale;
+  return ugb_masked_attention(dev, a);
+}
+
+}  // namespace
+
+extern "C" int32_t ugb_window_attend(ugb_device *dev, const ugb_slice *q, const ugb_slice *k, const ugb_slice *v, const ugb_slice *pos, ugb_slice *out, size_t b,
+                                     size_t t, size_t heads, size_t kv_heads, size_t dq, size_t dv, size_t t_max, size_t sinks, size_t window, float scale,
+                                     float out_scale) {
+  if (!dev) return UGB_ERR_INVALID;
+  UGB_REQUIRE(dev, window >= 1, UGB_ERR_INVALID, "window_attend: a window of no position");
+  return attend(dev, "window_attend", q, k, v, pos, nullptr, out, b, t, heads, kv_heads, dq, dv, t_max, sinks, window, scale, out_scale);
+}
+
+extern "C" int32_t ugb_tree_attend(ugb_device *dev, const ugb_slice *q, const ugb_slice *k, const ugb_slice *v, const ugb_slice *pos, const ugb_slice *parents,
+                                   ugb_slice *out, size_t b, size_t t, size_t heads, size_t kv_heads, size_t dq, size_t dv, size_t t_max, float scale,
+                                   float out_scale) {
+  if (!dev) return UGB_ERR_INVALID;
+  UGB_REQUIRE(dev, parents, UGB_ERR_INVALID, "tree_attend: null slice");
+  UGB_REQUIRE(dev, t <= UGB_TREE_MAX, UGB_ERR_UNSUPPORTED, "tree_attend: %zu nodes, at most %d", t, UGB_TREE_MAX);
+  return attend(dev, "tree_attend", q, k, v, pos, parents, out, b, t, heads, kv_heads, dq, dv, t_max, 0, t_max, scale, out_scale);
+}

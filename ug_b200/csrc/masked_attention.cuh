@@ -1,0 +1,58 @@
+// Grouped-query attention over a cache whose queries see a part of it: a sliding window beside the first positions, or the committed
+// positions and a node's ancestors.
+#pragma once
+#include "draft_rows.cuh"
+
+struct ugb_masked_attention_args {
+  bool f32;                  // T = f32, else bf16
+  const void *q;             // T [b][t][heads][dq]
+  const void *k, *v;         // T [b][kv_heads][t_max][dq / dv], the new positions' rows included
+  void *out;                 // T [b][t][heads][dv] times out_scale
+  const int *pos;            // [b] positions ahead of the new ones; -1: no sequence
+  const int *parents;        // [b][t]: a tree; null: a window
+  int b, t, heads, kv_heads, dq, dv, t_max;
+  int sinks, window;
+  float scale, out_scale;
+};
+
+// What a kernel needs to know of the mask.  Row r of a (sequence, key / value head) is query r / share of the block, head r % share of the
+// group, so that a tile of rows reads a tile of keys once for all heads of the group.
+struct ugb_mask {
+  const int *pos, *parents;
+  int t, t_max, sinks, window;
+};
+
+#ifdef __CUDACC__
+namespace ugb_masked {
+
+constexpr int KEYS = 64;     // of a tile
+
+__device__ __forceinline__ void raise_invalid(ugb_status_word *status, int detail) {
+  if (atomicCAS(&status->code, 0u, (unsigned)UGB_ERR_INVALID) == 0u) status->detail = (unsigned)detail;
+}
+
+// The keys that rows of queries i0 .. i1 of a sequence see: positions below `first` and from `from` on, up to `end` - 1, in tiles of KEYS
+// positions that start at multiples of KEYS.
+struct Span {
+  int first, from, end, first_tiles, from_tile, tiles;
+  __device__ __forceinline__ int key0(int tile) const { return (tile < first_tiles ? tile : from_tile + tile - first_tiles) * KEYS; }
+};
+template <bool TREE> __device__ __forceinline__ Span span_of(const ugb_mask &m, int pos, int i0, int i1) {
+  Span s;
+  s.end = pos + i1 + 1;
+  s.first = 0;
+  s.from = 0;
+  if constexpr (!TREE) {
+    s.from = max(0, pos + i0 - m.window + 1);
+    s.first = min(m.sinks, s.from);
+  }
+  s.first_tiles = (s.first + KEYS - 1) / KEYS;
+  s.from_tile = max(s.from / KEYS, s.first_tiles);
+  s.tiles = s.first_tiles + max(0, (s.end + KEYS - 1) / KEYS - s.from_tile);
+  return s;
+}
+
+}  // namespace ugb_masked
+#endif
+
+int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a);

@@ -353,3 +353,13 @@ class Device:
     def cache_keep(self, k, v, pos, path, count, b, kv_heads, dq, dv, t_max, most):
         """Moves the cache rows of accepted nodes up behind the committed positions."""
         self._check(lib.ugb_cache_keep(self._h, k._h, v._h, pos._h, path._h, count._h, b, kv_heads, dq, dv, t_max, most))
+
+    def tree_attend(self, q, k, v, pos, parents, out, b, t, heads, kv_heads, dq, dv, t_max, scale, out_scale=1.0):
+        """Grouped-query attention of drafted nodes over the committed positions and their ancestors."""
+        self._check(lib.ugb_tree_attend(self._h, q._h, k._h, v._h, pos._h, parents._h, out._h, b, t, heads, kv_heads, dq, dv, t_max, scale,
+                                        out_scale))
+
+    def window_attend(self, q, k, v, pos, out, b, t, heads, kv_heads, dq, dv, t_max, sinks, window, scale, out_scale=1.0):
+        """Grouped-query attention of new positions over the last ``window`` positions and the first ``sinks``."""
+        self._check(lib.ugb_window_attend(self._h, q._h, k._h, v._h, pos._h, out._h, b, t, heads, kv_heads, dq, dv, t_max, sinks, window,
+                                          scale, out_scale))
