@@ -1,7 +1,8 @@
 // Attention of new positions over a sliding window and the first positions of a cache, or over the cache and their ancestors in a
 // tree (ugb_window_attend, ugb_tree_attend; see masked_attention.cuh).
 //
-//   masked_attention_generic_kernel   f32, and heads that the tensor-core kernel does not take: plain FFMA over tiles of 64 keys
+//   masked_attention_tc_kernel        (masked_attention_tc.cu) bf16 heads of 64 or 128 values
+//   masked_attention_generic_kernel   f32, other heads, unaligned buffers: plain FFMA over tiles of 64 keys
 //   masked_combine_kernel             joins the slices of the keys that ran as separate CTAs
 //
 // One pass over the keys with the running maximum and sum of the softmax, in 32 bits, in powers of two.
@@ -17,16 +18,7 @@ using namespace ugb_masked;
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-struct Params {
-  const void *q, *k, *v;
-  void *out;
-  ugb_mask mask;
-  int heads, kv_heads, share, rows, dq, dv, splits;        // rows: t * share, of a sequence and key / value head
-  float scale, out_scale;                                  // scale: with log2(e)
-  float *part_o;                                           // [splits][b][kv_heads][rows][dv]
-  float2 *part_ml;                                         // (maximum, sum) alike
-  ugb_status_word *status;
-};
+using Params = ugb_masked_params;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -291,9 +283,11 @@ int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a
   // the most keys that a row of tiles can see: the position is on the device
   const long long reach = tree ? a.t_max : std::min<long long>(a.t_max, (long long)a.window + a.t + a.sinks);
   const int tiles = (int)((reach + KEYS - 1) / KEYS + 1), pairs = a.b * a.kv_heads;
+  const bool tc = ugb_masked_tc_takes(a);
   const int rm = p.rows <= 16 ? 1 : 4, row_tiles = (p.rows + 16 * rm - 1) / (16 * rm);
-  const size_t smem = generic_smem(a.dq, a.dv, 16 * rm);
-  p.splits = slices((long long)row_tiles * pairs, 2LL * dev->sm_count, tiles);
+  long long ctas = (long long)row_tiles * pairs, slots = 2LL * dev->sm_count;
+  if (tc) ugb_masked_tc_shape(dev, a, &ctas, &slots);
+  p.splits = slices(ctas, slots, tiles);
   const size_t n = (size_t)pairs * p.rows;
   void *work = nullptr;
   if (p.splits > 1) {
@@ -301,10 +295,16 @@ int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a
     p.part_o = (float *)work;
     p.part_ml = (float2 *)(p.part_o + (size_t)p.splits * n * a.dv);
   }
-  const dim3 grid((unsigned)row_tiles, (unsigned)pairs, (unsigned)p.splits);
-  const cudaError_t e = a.f32 ? launch_rows<float>(tree, rm, grid, smem, dev->stream, p) : launch_rows<__nv_bfloat16>(tree, rm, grid, smem, dev->stream, p);
-  int32_t rc = e != cudaSuccess ? ugb_fail(dev, UGB_ERR_CUDA, "launch of masked_attention_generic_kernel failed: %s", cudaGetErrorString(e))
-                                : ugb_after_launch(dev, "masked_attention_generic_kernel");
+  int32_t rc;
+  if (tc) {
+    rc = ugb_masked_tc_launch(dev, a, p);
+  } else {
+    const size_t smem = generic_smem(a.dq, a.dv, 16 * rm);
+    const dim3 grid((unsigned)row_tiles, (unsigned)pairs, (unsigned)p.splits);
+    const cudaError_t e = a.f32 ? launch_rows<float>(tree, rm, grid, smem, dev->stream, p) : launch_rows<__nv_bfloat16>(tree, rm, grid, smem, dev->stream, p);
+    rc = e != cudaSuccess ? ugb_fail(dev, UGB_ERR_CUDA, "launch of masked_attention_generic_kernel failed: %s", cudaGetErrorString(e))
+                          : ugb_after_launch(dev, "masked_attention_generic_kernel");
+  }
   if (rc == UGB_OK && p.splits > 1) {
     const dim3 rows((unsigned)((n + 7) / 8));
     if (a.f32) tree ? masked_combine_kernel<float, true><<<rows, 256, 0, dev->stream>>>(p, pairs) : masked_combine_kernel<float, false><<<rows, 256, 0, dev->stream>>>(p, pairs);

@@ -21,6 +21,16 @@ struct ugb_mask {
   const int *pos, *parents;
   int t, t_max, sinks, window;
 };
+struct ugb_masked_params {
+  const void *q, *k, *v;
+  void *out;
+  ugb_mask mask;
+  int heads, kv_heads, share, rows, dq, dv, splits;        // rows: t * share, of a sequence and key / value head
+  float scale, out_scale;                                  // scale: with log2(e)
+  float *part_o;                                           // of slices: [splits][b][kv_heads][rows][dv]
+  float2 *part_ml;                                         // (maximum, sum) alike
+  ugb_status_word *status;
+};
 
 #ifdef __CUDACC__
 namespace ugb_masked {
@@ -54,5 +64,10 @@ template <bool TREE> __device__ __forceinline__ Span span_of(const ugb_mask &m, 
 
 }  // namespace ugb_masked
 #endif
+
+// The tensor-core kernel (masked_attention_tc.cu).  Whether it takes a call; how many CTAs it makes of it and how many run at a time; its launch.
+bool ugb_masked_tc_takes(const ugb_masked_attention_args &a);
+void ugb_masked_tc_shape(const ugb_device *dev, const ugb_masked_attention_args &a, long long *ctas, long long *slots);
+int32_t ugb_masked_tc_launch(ugb_device *dev, const ugb_masked_attention_args &a, const ugb_masked_params &p);
 
 int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a);
