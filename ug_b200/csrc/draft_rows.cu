@@ -64,6 +64,25 @@ template <bool VEC> __device__ __forceinline__ void store8(float *p, const float
   }
 }
 
+// 8 values as they lie in memory, so that those of several heads can be on their way in few registers
+template <typename T> struct Piece { uint4 w[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ void fetch(const T *p, Piece<T> &r) {
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.w[i] = reinterpret_cast<const uint4 *>(p)[i];
+}
+__device__ __forceinline__ void unpack(const Piece<__nv_bfloat16> &r, float (&f)[8]) {
+  const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const Piece<float> &r, float (&f)[8]) {
+  f[0] = __uint_as_float(r.w[0].x); f[1] = __uint_as_float(r.w[0].y); f[2] = __uint_as_float(r.w[0].z); f[3] = __uint_as_float(r.w[0].w);
+  f[4] = __uint_as_float(r.w[1].x); f[5] = __uint_as_float(r.w[1].y); f[6] = __uint_as_float(r.w[1].z); f[7] = __uint_as_float(r.w[1].w);
+}
+
 __device__ __forceinline__ void raise(ugb_status_word *status, int detail) {
   if (atomicCAS(&status->code, 0u, (unsigned)UGB_ERR_INVALID) == 0u) status->detail = (unsigned)detail;
 }
@@ -79,13 +98,19 @@ struct InputParams {
   ugb_status_word *status;
 };
 
-// One CTA per node.  Groups of LANES lanes take a head each, 8 dimensions a lane (dim, vdim <= 8 LANES); the partner of a rotated
-// dimension is read again, from L1, where it belongs to another lane.
-template <typename T, int LANES, bool VEC>
-__global__ void __launch_bounds__(256)
-tree_inputs_kernel(InputParams p) {
-  __shared__ int up[UGB_TREE_MAX];
-  const int s = blockIdx.x / p.t, node = blockIdx.x % p.t;
+// How the partner of a rotated dimension is reached: pairs (2i, 2i + 1), both in a lane's piece; pairs (i, i + rot / 2) whose partners lie together,
+// in another piece (read again, from L1); value by value, which also goes for buffers that are not aligned.
+enum { INTERLEAVED, HALVES, SCATTERED };
+
+// A CTA takes `per` nodes of a sequence, one after the other through all their heads: groups of LANES lanes take a query or key head each, 8 dimensions a
+// lane (dim <= 8 LANES), two heads on their way at a time; the values are copied as they are.
+template <typename T, int LANES, int MODE>
+__global__ void __launch_bounds__(256, 4)
+tree_inputs_kernel(InputParams p, int per) {
+  constexpr int GROUPS = 256 / LANES;
+  constexpr bool VEC = MODE != SCATTERED;
+  __shared__ int up[UGB_TREE_MAX], at_s[UGB_TREE_MAX];
+  const int parts = (p.t + per - 1) / per, s = blockIdx.x / parts, first = blockIdx.x % parts * per, count = min(per, p.t - first);
   const int pos = p.pos[s];
   bool bad = false;
   for (int j = threadIdx.x; j < p.t; j += 256) {
@@ -99,81 +124,125 @@ tree_inputs_kernel(InputParams p) {
     if (threadIdx.x == 0) raise(p.status, bad ? s : pos);
     return;
   }
-  int at = pos;
-  for (int j = up[node]; j >= 0; j = up[j]) ++at;
-  const int half = p.rot / 2;
-  const float *cs = p.cos_ + (size_t)at * half, *sn = p.sin_ + (size_t)at * half;
-  const int all = p.heads + 2 * p.kv_heads, turned = p.heads + p.kv_heads;
-  const T *pre = (const T *)p.pre + ((size_t)s * p.t + node) * ((size_t)turned * p.dim + (size_t)p.kv_heads * p.vdim);
-  const int group = threadIdx.x / LANES, c0 = (threadIdx.x % LANES) * 8;
-  for (int h0 = 0; h0 < all; h0 += 256 / LANES) {          // all lanes of a warp stay together for the sums
-    const int h = h0 + group;
-    const bool rotated = h < turned;
-    const int width = rotated ? p.dim : p.vdim;
-    const bool on = h < all && c0 < width;
-    const T *x = pre + (rotated ? (size_t)h * p.dim : (size_t)turned * p.dim + (size_t)(h - turned) * p.vdim);
-    float f[8];
+  if ((int)threadIdx.x < count) {
+    int at = pos;
+    for (int j = up[first + threadIdx.x]; j >= 0; j = up[j]) ++at;
+    at_s[threadIdx.x] = at;
+  }
+  const int half = p.rot / 2, turned = p.heads + p.kv_heads;
+  const size_t ld = (size_t)turned * p.dim + (size_t)p.kv_heads * p.vdim, row0 = (size_t)s * p.t + first;
+  const T *pre = (const T *)p.pre + row0 * ld;
+  {   // values
+    constexpr int N = VEC ? 8 : 1;
+    const int pieces = p.kv_heads * p.vdim / N, width = p.vdim / N;
+    for (int i = threadIdx.x; i < count * pieces; i += 256) {
+      const int node = i / pieces, j = i - node * pieces, h = j / width, c = (j - h * width) * N;
+      const T *x = pre + node * ld + (size_t)turned * p.dim + (size_t)h * p.vdim + c;
+      T *y = (T *)p.v + (((size_t)s * p.kv_heads + h) * p.t_max + pos + first + node) * p.vdim + c;
+      if constexpr (VEC) {
+        Piece<T> w;
+        fetch(x, w);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = 0.f;
-    if (on) load8<VEC>(x + c0, f);
-    if (on && rotated) {
-      if (p.interleaved) {                                 // pairs (2i, 2i + 1): both in this lane
-#pragma unroll
-        for (int e = 0; e < 8; e += 2)
-          if (c0 + e < p.rot) {
-            const float c = cs[(c0 + e) / 2], n = sn[(c0 + e) / 2], a = f[e], b = f[e + 1];
-            f[e] = a * c - b * n;
-            f[e + 1] = b * c + a * n;
-          }
-      } else if (VEC && half % 8 == 0) {                   // pairs (i, i + half): all 8 partners lie together, on one side
-        if (c0 < p.rot) {
-          const bool low = c0 < half;
-          const int i = low ? c0 : c0 - half;
-          float o[8], c[8], n[8];
-          load8<VEC>(x + (low ? c0 + half : i), o);
-          load8<VEC>(cs + i, c);
-          load8<VEC>(sn + i, n);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = low ? f[e] * c[e] - o[e] * n[e] : f[e] * c[e] + o[e] * n[e];
-        }
+        for (int e = 0; e < (int)sizeof(T) / 2; ++e) reinterpret_cast<uint4 *>(y)[e] = w.w[e];
       } else {
+        *y = *x;
+      }
+    }
+  }
+  __syncthreads();
+  const int group = threadIdx.x / LANES, c0 = (threadIdx.x % LANES) * 8, total = count * turned;
+  const bool on_lane = c0 < p.dim, turns = c0 < p.rot, low = c0 < half;
+  const int partner = low ? c0 + half : c0 - half, table = MODE == INTERLEAVED ? c0 / 2 : low ? c0 : c0 - half;
+  const float inv_dim = 1.0f / (float)p.dim;
+  int node = 0, h = group;                                 // of this group's next head
+  while (h >= turned) { h -= turned; ++node; }
+  for (int w0 = 0; w0 < total; w0 += 2 * GROUPS) {         // all lanes of a warp stay together for the sums
+    Piece<T> own[2], other[2];
+    int nodes[2], hs[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int d = c0 + e;
-          if (d < p.rot) {
-            const bool low = d < half;
-            const int i = low ? d : d - half;
-            const float o = to_f32(x[low ? d + half : i]);
-            f[e] = low ? f[e] * cs[i] - o * sn[i] : f[e] * cs[i] + o * sn[i];
+    for (int k = 0; k < 2; ++k) {
+      nodes[k] = node;
+      hs[k] = h;
+      const T *x = pre + node * ld + (size_t)h * p.dim;
+      if constexpr (VEC)
+        if (on_lane && node < count) {
+          fetch(x + c0, own[k]);
+          if (MODE == HALVES && turns) fetch(x + partner, other[k]);
+        }
+      h += GROUPS;
+      while (h >= turned) { h -= turned; ++node; }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const bool on = on_lane && nodes[k] < count;
+      float f[8], o[8], c[8], n[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = 0.f;
+      if (on) {
+        const int at = at_s[nodes[k]];
+        const float *cs = p.cos_ + (size_t)at * half, *sn = p.sin_ + (size_t)at * half;
+        const T *x = pre + nodes[k] * ld + (size_t)hs[k] * p.dim;
+        if constexpr (VEC) unpack(own[k], f);
+        else load8<false>(x + c0, f);
+        if constexpr (MODE == SCATTERED) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int d = c0 + e;
+            if (d < p.rot) {
+              const bool one = p.interleaved ? d % 2 == 0 : d < half;
+              const int i = p.interleaved ? d / 2 : one ? d : d - half, other_d = p.interleaved ? d ^ 1 : one ? d + half : d - half;
+              const float a = to_f32(x[d]), b = to_f32(x[other_d]);
+              f[e] = one ? a * cs[i] - b * sn[i] : a * cs[i] + b * sn[i];
+            }
+          }
+        } else if (turns) {
+          if constexpr (MODE == INTERLEAVED) {             // the table's rows start anywhere
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+              if (c0 + e < p.rot) {
+                c[0] = cs[table + e / 2];
+                n[0] = sn[table + e / 2];
+                const float a = f[e], b = f[e + 1];
+                f[e] = a * c[0] - b * n[0];
+                f[e + 1] = b * c[0] + a * n[0];
+              }
+          } else {
+            unpack(other[k], o);
+            load8<true>(cs + table, c);
+            load8<true>(sn + table, n);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = f[e] * c[e] + (low ? -o[e] : o[e]) * n[e];
           }
         }
       }
-    }
-    if (p.norm) {                                          // sum of squares over the lanes of the head, in 32 bits
-      float ss = 0.f;
+      if (p.norm) {                                        // sum of squares over the lanes of the head, in 32 bits
+        float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
 #pragma unroll
-      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (rotated) {
-        const float r = 1.0f / sqrtf(ss / (float)p.dim + p.eps);
+        for (int d = LANES / 2; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+        const float r = rsqrtf(ss * inv_dim + p.eps);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] *= r;
       }
+      if (!on) continue;
+      const bool query = hs[k] < p.heads;
+      T *y = query ? (T *)p.q + ((row0 + nodes[k]) * p.heads + hs[k]) * p.dim
+                   : (T *)p.k + (((size_t)s * p.kv_heads + (hs[k] - p.heads)) * p.t_max + pos + first + nodes[k]) * p.dim;
+      store8<VEC>(y + c0, f);
     }
-    if (!on) continue;
-    const size_t row = pos + node;
-    if (h < p.heads) store8<VEC>((T *)p.q + (((size_t)s * p.t + node) * p.heads + h) * p.dim + c0, f);
-    else if (rotated) store8<VEC>((T *)p.k + (((size_t)s * p.kv_heads + (h - p.heads)) * p.t_max + row) * p.dim + c0, f);
-    else store8<VEC>((T *)p.v + (((size_t)s * p.kv_heads + (h - turned)) * p.t_max + row) * p.vdim + c0, f);
   }
 }
 
-template <typename T, bool VEC> void launch_inputs(dim3 grid, cudaStream_t st, const InputParams &p) {
-  const int widest = p.dim > p.vdim ? p.dim : p.vdim;
-  if (widest <= 64) tree_inputs_kernel<T, 8, VEC><<<grid, 256, 0, st>>>(p);
-  else if (widest <= 128) tree_inputs_kernel<T, 16, VEC><<<grid, 256, 0, st>>>(p);
-  else tree_inputs_kernel<T, 32, VEC><<<grid, 256, 0, st>>>(p);
+template <typename T, int MODE> void launch_inputs(dim3 grid, cudaStream_t st, const InputParams &p, int per) {
+  if (p.dim <= 64) tree_inputs_kernel<T, 8, MODE><<<grid, 256, 0, st>>>(p, per);
+  else if (p.dim <= 128) tree_inputs_kernel<T, 16, MODE><<<grid, 256, 0, st>>>(p, per);
+  else tree_inputs_kernel<T, 32, MODE><<<grid, 256, 0, st>>>(p, per);
+}
+template <typename T> void launch_inputs(int mode, dim3 grid, cudaStream_t st, const InputParams &p, int per) {
+  if (mode == INTERLEAVED) launch_inputs<T, INTERLEAVED>(grid, st, p, per);
+  else if (mode == HALVES) launch_inputs<T, HALVES>(grid, st, p, per);
+  else launch_inputs<T, SCATTERED>(grid, st, p, per);
 }
 
 // ------------------------------------------------------------------ keep ----
@@ -257,11 +326,14 @@ extern "C" int32_t ugb_tree_inputs(ugb_device *dev, const ugb_slice *pre, const 
   p.parents = (const int *)parents->ptr; p.q = q->ptr; p.k = kcache->ptr; p.v = vcache->ptr; p.t = (int)t; p.heads = (int)heads;
   p.kv_heads = (int)kv_heads; p.dim = (int)dim; p.vdim = (int)vdim; p.rot = (int)rot_dims; p.interleaved = interleaved != 0;
   p.norm = qk_norm != 0; p.eps = eps; p.t_max = (int)t_max; p.status = dev->status_dev;
-  const dim3 grid((unsigned)(b * t));
-  // rows start at multiples of 8 values: aligned buffers make every piece of 8 aligned (the tables' too, where half % 8 == 0 asks for it)
+  // several nodes share the look at the tree where there are more than fill the GPU
+  const size_t fill = 4 * (size_t)dev->sm_count, per = (b * t + fill - 1) / fill < t ? (b * t + fill - 1) / fill : t;
+  const dim3 grid((unsigned)(b * ((t + per - 1) / per)));
+  // rows start at multiples of 8 values: aligned buffers make every piece of 8 aligned (the tables' too, where rot % 16 == 0)
   const bool vec = aligned16(pre->ptr) && aligned16(q->ptr) && aligned16(kcache->ptr) && aligned16(vcache->ptr) && aligned16(cos_->ptr) && aligned16(sin_->ptr);
-  if (q->dtype == UGB_F32) vec ? launch_inputs<float, true>(grid, dev->stream, p) : launch_inputs<float, false>(grid, dev->stream, p);
-  else vec ? launch_inputs<__nv_bfloat16, true>(grid, dev->stream, p) : launch_inputs<__nv_bfloat16, false>(grid, dev->stream, p);
+  const int mode = !vec || (!interleaved && rot_dims % 16) ? SCATTERED : interleaved ? INTERLEAVED : HALVES;
+  if (q->dtype == UGB_F32) launch_inputs<float>(mode, grid, dev->stream, p, (int)per);
+  else launch_inputs<__nv_bfloat16>(mode, grid, dev->stream, p, (int)per);
   return ugb_after_launch(dev, "tree_inputs_kernel");
 }
 
