@@ -95,6 +95,7 @@ def test_masked_logits(dev, vocab):
     x[7, 3] = x[7, 5] = np.inf
     x[8] = np.inf
     x[9, 2:] = -np.inf
+    x[3, 1::3] = -np.inf
     u = np.full(10, 0.6)
     for settings in (dict(), dict(top_k=4), dict(top_p=0.8), dict(top_k=vocab - 1, top_p=0.9, min_p=0.05), dict(temperature=0.0)):
         check(dev, x, u, **{n: [v] * 10 for n, v in settings.items()})
@@ -105,7 +106,7 @@ def test_wide_range_of_values(dev):
     x = np.concatenate([s * 2.0 ** np.arange(-126, 12) for s in (-1, 1)]).astype(np.float32)[None].repeat(8, 0)
     x[4:] = np.nextafter(np.float32(8), np.float32(9)) + np.arange(x.shape[1], dtype=np.float32) * np.float32(2.0 ** -20)
     u = np.tile([0.1, 0.5, 0.9, 0.999], 2)
-    for settings in (dict(top_k=10), dict(temperature=300.0, top_p=0.9), dict(temperature=1e4, top_k=200, top_p=0.7)):
+    for settings in (dict(temperature=1e20), dict(temperature=1e-45, top_p=0.5), dict(top_k=10), dict(temperature=300.0, top_p=0.9), dict(temperature=1e4, top_k=200, top_p=0.7)):
         check(dev, x, u, **{n: [v] * 8 for n, v in settings.items()})
 
 
@@ -138,7 +139,7 @@ def test_a_row_is_the_same_in_any_batch(dev):
         assert prob.to_vec().tolist() == [float(p.to_vec()[0]) for _, p in one] * times
 
 
-@pytest.mark.parametrize("name,value", [("temperature", -0.5), ("temperature", np.nan), ("temperature", np.inf), ("top_k", -1), ("top_p", 0.0), ("top_p", np.nan),
+@pytest.mark.parametrize("name,value", [("temperature", -0.5), ("temperature", np.nan), ("temperature", np.inf), ("temperature", 2e20), ("top_k", -1), ("top_p", 0.0), ("top_p", np.nan),
                                         ("min_p", -0.1), ("min_p", 1.5), ("min_p", np.nan), ("u", 1.0), ("u", -0.1), ("u", np.nan)])
 def test_values_outside_their_range(dev, name, value):
     """The row is left as it was, the others are done."""

@@ -32,7 +32,8 @@ typedef unsigned long long u64;
 constexpr int THREADS = 512, WARPS = THREADS / 32, CLUSTER_MAX = 8;
 constexpr int STEPS = 1024, RANKED = 256;
 constexpr float STEPS_PER_T = 32.0f;                       // 1024 steps reach to exp(-32) < 2^-45: what is beyond weighs nothing
-constexpr double UNIT = 17592186044416.0;                  // 2^44
+constexpr int POWERS = 256;
+constexpr float LOWEST_ABOVE = -3.4028232e38f;             // the second lowest value
 
 struct Params {
   const void *logits;
@@ -58,7 +59,7 @@ __device__ __forceinline__ u64 peer_u64(uint32_t addr, int rank) {
 
 struct Shared {
   u64 warp_sum[WARPS];
-  double power[64];                                        // 2^(i / 64)
+  double power[POWERS];                                    // 2^(i / POWERS)
   u64 hist[STEPS];
   u64 in_step[RANKED], before_step[RANKED];                // tokens by place()
   u64 ranked[RANKED], sorted[RANKED];
@@ -69,27 +70,35 @@ struct Shared {
   u64 pick[4];
 };
 
-// Weights by Tang's table method for the exponential: e^y = 2^(n / 64) e^r, |r| <= ln 2 / 128, e^r by its series to r^4 (4e-14).
+// Weights, in units of 2^-44 of the best one's, by Tang's table method for the exponential: with t = 256 (x - best) log2(e) / T = n + f, |f| <= 1/2,
+// 2^(t / 256) is a power from the table, shifted, times 2^(f / 256) by its series to f^3 (1.4e-13 of the value).
 struct Weights {
-  float best;
-  double inv_t;
+  float best, lowest;
+  double best_d, k;
   const double *power;
-  __device__ __forceinline__ double exact(float x) const {
-    if (x == best) return 1.0;
-    const double y = ((double)x - (double)best) * inv_t;
-    if (!(y > -40.0)) return 0.0;                          // below half a unit
-    const double shifted = fma(y, 92.332482616893656877, 6755399441055744.0);   // 64 / ln 2; + 1.5 * 2^52: the integer is in the low bits
-    const int n = __double2loint(shifted);
-    const double r = fma(shifted - 6755399441055744.0, -0.010830424696249145, y);
-    double e = fma(r, 1.0 / 24.0, 1.0 / 6.0);
-    e = fma(e, r, 0.5);
-    e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0) * power[n & 63];
-    return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
+  __device__ __forceinline__ Weights(float best_, float temperature, const double *power_) : best(best_), best_d(best_), power(power_) {
+    const float below = nextafterf(best, -INFINITY);
+    // where the next smaller value weighs nothing already, a larger T does not change that, and keeps t within the integers
+    const double t = fmax((double)temperature, (best_d - (double)below) / 64.0);
+    k = POWERS * 1.4426950408889634 / t;
+    lowest = fmaxf(fminf(best - 64.0f * temperature, below), -3.4028234e38f);         // exp(-42) and less from here on, rounding included; -inf too
+    per_unit = (float)fmin(STEPS_PER_T / t, 3.0e38);
   }
-  // in units of 2^-44: the low bits of the sum with 2^8, whose last place that is
-  __device__ __forceinline__ u64 of(double w) const { return (u64)(__double_as_longlong(w + 256.0) - __double_as_longlong(256.0)); }
-  __device__ __forceinline__ u64 units(float x) const { return of(exact(x)); }
+  float per_unit;                                          // steps of the histogram per unit of the logit
+  __device__ __forceinline__ u64 units(float x) const {
+    const double d = (double)fmaxf(x, lowest) - best_d;
+    const double shifted = fma(d, k, 6755399441055744.0);  // + 1.5 * 2^52: the integer is in the low bits
+    const double f = fma(d, k, 6755399441055744.0 - shifted);
+    const int n = __double2loint(shifted);
+    constexpr double C = 0.69314718055994531 / POWERS;
+    double e = fma(f, C * C * C / 6.0, C * C / 2.0);
+    e = fma(e, f, C);
+    e = fma(e, f, 1.0);
+    const double w = power[n & (POWERS - 1)];
+    // + 2^8, whose last place is 2^-44
+    e = fma(__hiloint2double(__double2hiint(w) + ((n >> 8) << 20), __double2loint(w)), e, 256.0);
+    return ((u64)(uint32_t)(__double2hiint(e) - 0x40700000) << 32) | (uint32_t)__double2loint(e);
+  }
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -119,7 +128,7 @@ template <typename T> struct Row {
   const T *x;
   int base, len, rank, size, seg;
   __device__ __forceinline__ float at(int i) const { return (float)x[i]; }
-  // f(index in the CTA, logit) for this thread's share, four loads ahead
+  // f(index in the CTA, logit) for this thread's share, four at a time
   template <typename F> __device__ __forceinline__ void each(F f) const {
     const int from = min(len, (int)threadIdx.x * seg), to = min(len, ((int)threadIdx.x + 1) * seg);
     int i = from;
@@ -193,17 +202,17 @@ __device__ int find_index(const Row<T> &r, Shared &sh, u64 target, u64 mine, u64
 struct ByDistance {                                        // from the best logit; rounding keeps the order
   float best, per_unit;
   __device__ __forceinline__ int of(float x) const {
-    const float d = x == best ? 0.0f : (best - x) * per_unit;
+    const float d = (best - x) * per_unit;
     return d < (float)STEPS ? (int)d : STEPS;
   }
+  __device__ __forceinline__ bool behind(float x, int step) const { return (best - x) * per_unit >= (float)(step + 1); }
 };
 struct ByKey {                                             // of the keys min .. max
-  uint32_t min, max;
+  uint32_t max;
   int shift;
-  __device__ __forceinline__ int of(float x) const {
-    const uint32_t k = key_of(x);
-    return k > max ? -1 : k < min ? STEPS : (int)((max - k) >> shift);
-  }
+  float low, high;                                         // their values
+  __device__ __forceinline__ int of(float x) const { return x > high ? -1 : x < low ? STEPS : (int)((max - key_of(x)) >> shift); }
+  __device__ __forceinline__ bool behind(float x, int step) const { return x < low || (x <= high && (int)((max - key_of(x)) >> shift) > step); }
 };
 
 // Adds weigh(logit, index) of the tokens of all steps to the histogram, over the cluster, and finds the step in which the running sum reaches the
@@ -275,20 +284,24 @@ __device__ int find_step(const Row<T> &r, Shared &sh, const S &steps, F weigh, G
 }
 
 // Lists the tokens of step `in` and (before) of the steps before it, up to RANKED of each kind, every CTA its own.  n_in, n_before: how many there
-// are in the cluster (more than RANKED: that many or more); min, max: the keys of those in the step.
+// are in the cluster (more than RANKED: that many or more); mine: this thread's tokens of the step; min, max: the keys of the step's.
 template <typename T, typename S, typename F>
-__device__ void gather(const Row<T> &r, Shared &sh, const S &steps, int in, bool before, F valid, int slot, int *n_in, int *n_before, uint32_t *min_key, uint32_t *max_key) {
-  uint32_t lo = 0xffffffffu, hi = 0;
+__device__ void gather(const Row<T> &r, Shared &sh, const S &steps, int in, bool before, F valid, int slot, int *n_in, int *n_before, int *mine, uint32_t *min_key,
+                       uint32_t *max_key) {
+  float low = INFINITY, high = -INFINITY;
+  int count = 0;
   r.each([&](int i, float x) {
-    const int at = steps.of(x);
-    if (at < 0 || at > in || at == STEPS || (at < in && !before) || !valid(x, r.base + i)) return;
-    const uint32_t k = key_of(x);
-    if (at == in) { lo = min(lo, k); hi = max(hi, k); }
-    int *n = at == in ? &sh.n_in : &sh.n_before;
+    if (steps.behind(x, in) || !valid(x, r.base + i)) return;
+    const bool here = steps.of(x) == in;
+    if (here) { low = fminf(low, x); high = fmaxf(high, x); ++count; }
+    if (!here && !before) return;
+    int *n = here ? &sh.n_in : &sh.n_before;
     if (*reinterpret_cast<volatile int *>(n) > RANKED) return;
     const int j = atomicAdd(n, 1);
-    if (j < RANKED) (at == in ? sh.in_step : sh.before_step)[j] = place(k, r.base + i);
+    if (j < RANKED) (here ? sh.in_step : sh.before_step)[j] = place(key_of(x), r.base + i);
   });
+  *mine = count;
+  uint32_t lo = count ? key_of(low) : 0xffffffffu, hi = count ? key_of(high) : 0;
   lo = __reduce_min_sync(0xffffffffu, lo);
   hi = __reduce_max_sync(0xffffffffu, hi);
   if ((threadIdx.x & 31) == 0) {
@@ -382,106 +395,119 @@ sample_kernel(Params p, int size) {
   const float u = p.u[row];
   const int top_k = p.top_k ? p.top_k[row] : 0;
   // negated comparisons: a NaN is refused
-  if (!(temperature >= 0.0f) || isinf(temperature) || top_k < 0 || !(top_p > 0.0f) || !(min_p >= 0.0f && min_p <= 1.0f) || !(u >= 0.0f && u < 1.0f)) {
+  if (!(temperature >= 0.0f && temperature <= 1e20f) || top_k < 0 || !(top_p > 0.0f) || !(min_p >= 0.0f && min_p <= 1.0f) || !(u >= 0.0f && u < 1.0f)) {
     if (me == 0 && threadIdx.x == 0 && atomicCAS(&p.status->code, 0u, (unsigned)UGB_ERR_INVALID) == 0u) p.status->detail = (unsigned)row;
     return;                                                // the whole cluster: the row is left as it was
   }
   const T *g = (const T *)p.logits + (long long)row * p.ld + r.base;
+  // NaN becomes -inf, which is no candidate: a maximum ignores it
   float best = -INFINITY;
-  int at = 0x7fffffff;
-  auto take = [&](float v, int i) {
-    v = v != v ? -INFINITY : v;                            // a NaN is no candidate
-    x[i] = (T)v;
-    if (v > best || (v == best && i < at)) { best = v; at = i; }
-  };
   constexpr int PER = 16 / (int)sizeof(T);
   if (((uintptr_t)g & 15) == 0) {
     for (int i = threadIdx.x * PER; i + PER <= r.len; i += THREADS * PER) {
-      const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(g + i));
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      uint4 v = __ldcs(reinterpret_cast<const uint4 *>(g + i));
+      uint32_t *w = &v.x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if constexpr (sizeof(T) == 4) take(__uint_as_float(w[j]), i + j);
-        else {
-          take(__uint_as_float(w[j] << 16), i + 2 * j);
-          take(__uint_as_float(w[j] & 0xffff0000u), i + 2 * j + 1);
+        if constexpr (sizeof(T) == 4) {
+          const float f = fmaxf(__uint_as_float(w[j]), -INFINITY);
+          w[j] = __float_as_uint(f);
+          best = fmaxf(best, f);
+        } else {
+          const float a = fmaxf(__uint_as_float(w[j] << 16), -INFINITY), b = fmaxf(__uint_as_float(w[j] & 0xffff0000u), -INFINITY);
+          w[j] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+          best = fmaxf(best, fmaxf(a, b));
         }
       }
+      *reinterpret_cast<uint4 *>(x + i) = v;
     }
-    for (int i = r.len / PER * PER + threadIdx.x; i < r.len; i += THREADS) take(load1(g + i), i);
+    for (int i = r.len / PER * PER + threadIdx.x; i < r.len; i += THREADS) {
+      const float f = fmaxf(load1(g + i), -INFINITY);
+      x[i] = (T)f;
+      best = fmaxf(best, f);
+    }
   } else {
-    for (int i = threadIdx.x; i < r.len; i += THREADS) take(load1(g + i), i);
+    for (int i = threadIdx.x; i < r.len; i += THREADS) {
+      const float f = fmaxf(load1(g + i), -INFINITY);
+      x[i] = (T)f;
+      best = fmaxf(best, f);
+    }
   }
-  if (threadIdx.x < 64) sh.power[threadIdx.x] = exp2(threadIdx.x / 64.0);
-  u64 top = at == 0x7fffffff ? 0 : place(key_of(best), r.base + at);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (threadIdx.x < POWERS) sh.power[threadIdx.x] = exp2(threadIdx.x / (double)POWERS);
+  uint32_t top = __reduce_max_sync(0xffffffffu, key_of(best));
   if ((threadIdx.x & 31) == 0) sh.warp_sum[threadIdx.x >> 5] = top;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 0; w < WARPS; ++w) top = max(top, sh.warp_sum[w]);
-    sh.slot[0] = top;
+  if (threadIdx.x < 32) {
+    top = __reduce_max_sync(0xffffffffu, threadIdx.x < WARPS ? (uint32_t)sh.warp_sum[threadIdx.x] : 0);
+    if (threadIdx.x == 0) sh.slot[0] = top;
   }
   cluster_sync_all();
   top = 0;
 #pragma unroll
   for (int c = 0; c < CLUSTER_MAX; ++c)
-    if (c < size) top = max(top, peer_u64(smem_u32(&sh.slot[0]), c));
-  Weights weights;
-  weights.best = value_of(key_at(top));
-  weights.inv_t = 1.0 / (double)temperature;
-  weights.power = sh.power;
-  int token = index_at(top);
-  float prob = 1.0f;
-  if (weights.best == -INFINITY) {                         // nothing to choose from
-    token = -1;
-    prob = 0.0f;
-  } else if (temperature > 0.0f) {
-    const double low = (double)min_p;
+    if (c < size) top = max(top, (uint32_t)peer_u64(smem_u32(&sh.slot[0]), c));
+  best = value_of(top);
+  int token = -1;
+  float prob = 0.0f;
+  if (best == -INFINITY) {                                 // nothing to choose from
+  } else if (temperature == 0.0f) {
+    u64 mine = 0, before;                                  // the first of the best ones
+    r.each([&](int, float v) { mine += v == best ? 1 : 0; });
+    cluster_sum(block_sum(mine, sh), r, sh, 11, &before);
+    token = find_index(r, sh, 0, mine, before, [&](float v, int) { return (u64)(v == best ? 1 : 0); }, 12, nullptr);
+    prob = 1.0f;
+  } else {
+    if (best == INFINITY || best < LOWEST_ABOVE) {         // infinitely better than the others, or these are -inf: equal ones weigh the same
+      r.each([&](int i, float v) { x[i] = (T)(v == best ? 0.0f : -INFINITY); });          // every thread reads its own share only
+      best = 0.0f;
+    }
+    const Weights weights(best, temperature, sh.power);
+    const u64 low = min_p > 0.0f ? (u64)ceil((double)min_p * 17592186044416.0) : 0;       // 2^44 units
     auto share_of = [&](u64 sum) { return min(sum, max((u64)1, (u64)ceil((double)top_p * (double)sum))); };
     auto drawn = [&](u64 sum) { return min(sum - 1, __umul64hi((u64)((double)u * 18446744073709551616.0), sum)); };
     const bool by_k = top_k > 0 && top_k < p.vocab, by_p = top_p < 1.0f;
     // behind this step everything weighs less than min_p (a step more, for the rounding of both sides)
     const int low_step = min_p > 0.0f ? min(STEPS - 1, (int)(-logf(min_p) * STEPS_PER_T) + 1) : STEPS - 1;
-    u64 cut = 0;                                           // tokens of this place and the ones before it stay
-    auto stays = [&](float v, int i) { return place(key_of(v), i) >= cut; };
+    float cut = -INFINITY;                                 // tokens above it stay, and of those at it the ones up to index `last`
+    int last = p.vocab;
+    auto stays = [&](float v, int i) { return v > cut || (v == cut && i <= last); };
     // The choice among n ranked tokens, all that can be chosen; sum: what top_p is a share of, unless that is the first top_k.  CTA 0 alone.
     auto finish = [&](int n, bool first_k, u64 sum) {
       sort_ranked(sh, n);
       const u64 e = (int)threadIdx.x < n ? sh.sorted[threadIdx.x] : 0;
-      const double w = (int)threadIdx.x < n ? weights.exact(value_of(key_at(e))) : 0.0;
+      const u64 units = (int)threadIdx.x < n ? weights.units(value_of(key_at(e))) : 0;
       bool in = (int)threadIdx.x < n && (!first_k || (int)threadIdx.x < top_k);
-      u64 units = in ? weights.of(w) : 0;
       if (by_p) {
-        if (first_k) sum = block_sum(units, sh);
-        const u64 before = block_before(units, sh);        // a barrier: by every thread, whatever `in` is
+        const u64 w = in ? units : 0;
+        if (first_k) sum = block_sum(w, sh);
+        const u64 before = block_before(w, sh);            // a barrier: by every thread, whatever `in` is
         in = in && before < share_of(sum);
       }
-      in = in && w >= low;
+      in = in && units >= low;
       // what stays is a beginning: its tokens by index, the lowest first
       const int m = __syncthreads_count(in);
       if (in) sh.ranked[threadIdx.x] = ((u64)(uint32_t)~(uint32_t)index_at(e) << 32) | key_at(e);
       __syncthreads();
       sort_ranked(sh, m);
       const u64 f = (int)threadIdx.x < m ? sh.sorted[threadIdx.x] : 0;
-      units = (int)threadIdx.x < m ? weights.units(value_of((uint32_t)f)) : 0;
-      const u64 all = block_sum(units, sh), before = block_before(units, sh), target = drawn(all);
-      if (before <= target && target < before + units) {
+      const u64 w = (int)threadIdx.x < m ? weights.units(value_of((uint32_t)f)) : 0;
+      const u64 all = block_sum(w, sh), before = block_before(w, sh), target = drawn(all);
+      if (before <= target && target < before + w) {
         p.tokens[row] = (int)~(uint32_t)(f >> 32);
-        if (p.prob) p.prob[row] = (float)((double)units / (double)all);
+        if (p.prob) p.prob[row] = (float)((double)w / (double)all);
       }
     };
     bool done = false;
     // Finds the cut at which the running sum of weigh over the tokens that stay reaches a target, or makes the choice.
     auto narrow = [&](auto weigh, auto goal, bool first_k, int slot) {
-      ByDistance steps{weights.best, STEPS_PER_T / temperature};
+      const ByDistance steps{best, weights.per_unit};
       u64 above, within, whole, target;
-      int n_in, n_before;
+      int n_in, n_before, own;
       uint32_t key_min, key_max;
       const int step = find_step(r, sh, steps, weigh, goal, &above, &within, &whole, &target);
       const bool beyond = step == STEPS;                   // fewer tokens weigh anything than top_k: all of them stay
       const int in = min(beyond ? STEPS - 1 : step, by_p && first_k ? STEPS - 1 : low_step);   // top_p after top_k needs all the first top_k
-      gather(r, sh, steps, in, true, stays, slot, &n_in, &n_before, &key_min, &key_max);
+      gather(r, sh, steps, in, true, stays, slot, &n_in, &n_before, &own, &key_min, &key_max);
       if (n_in + n_before <= RANKED) {
         if (me == 0) collect(r, sh, slot, true);
         cluster_sync_all();                                // the others leave
@@ -498,25 +524,26 @@ sample_kernel(Params p, int size) {
           const u64 w = (int)threadIdx.x < n_in ? weigh(value_of(key_at(e)), index_at(e)) : 0, sum = above + block_before(w, sh);
           if (sum < target && target <= sum + w) sh.pick[3] = e;
           __syncthreads();
-          cut = sh.pick[3];
+          cut = value_of(key_at(sh.pick[3]));
+          last = index_at(sh.pick[3]);
           break;
         }
         if (key_min == key_max) {                          // equal logits, which weigh the same: by index
           const u64 w = first_k ? 1 : weights.units(value_of(key_min)), ties = (target - above + w - 1) / w;
-          auto tied = [&](float v, int i) { return (u64)(key_of(v) == key_min && stays(v, i) ? 1 : 0); };
-          u64 mine = 0, before;
-          r.each([&](int i, float v) { mine += tied(v, r.base + i); });
-          cluster_sum(block_sum(mine, sh), r, sh, slot + 2, &before);
-          const int last = find_index(r, sh, ties - 1, mine, before, tied, slot + 3, nullptr);
-          cut = place(key_min, last);
+          const float level = value_of(key_min);
+          auto tied = [&](float v, int i) { return (u64)(v == level && stays(v, i) ? 1 : 0); };
+          u64 before;
+          cluster_sum(block_sum((u64)own, sh), r, sh, slot + 2, &before);
+          last = find_index(r, sh, ties - 1, (u64)own, before, tied, slot + 3, nullptr);
+          cut = level;
           break;
         }
-        ByKey keys{key_min, key_max, max(0, 22 - __clz(key_max - key_min))};     // (max - min) >> shift < 1024
+        const ByKey keys{key_max, max(0, 22 - __clz(key_max - key_min)), value_of(key_min), value_of(key_max)};       // (max - min) >> shift < 1024
         const u64 over = above;
         const int at = find_step(r, sh, keys, weigh, [&](u64) { return target - over; }, &above, &within, &whole, &target);
         above += over;
         target += over;
-        gather(r, sh, keys, at, false, stays, slot, &n_in, &n_before, &key_min, &key_max);
+        gather(r, sh, keys, at, false, stays, slot, &n_in, &n_before, &own, &key_min, &key_max);
       }
       __syncthreads();
     };
@@ -524,8 +551,8 @@ sample_kernel(Params p, int size) {
     if (!done && by_p) narrow([&](float v, int i) { return stays(v, i) ? weights.units(v) : (u64)0; }, share_of, false, 6);
     if (done) return;
     auto kept = [&](float v, int i) -> u64 {
-      const double w = weights.exact(v);
-      return stays(v, i) && w >= low ? weights.of(w) : 0;
+      const u64 w = weights.units(v);
+      return stays(v, i) && w >= low ? w : 0;
     };
     u64 mine = 0, before, w;
     r.each([&](int i, float v) { mine += kept(v, r.base + i); });
@@ -561,7 +588,7 @@ int32_t ugb_sample_rows(ugb_device *dev, const ugb_sample_args &a) {
   p.prob = a.prob; p.rows = a.rows; p.vocab = a.vocab; p.ld = a.ld; p.status = dev->status_dev;
   // CTAs of a row: so many that the GPU is full, and that a row leaves room for three CTAs on an SM
   int size = 1;
-  while (size < CLUSTER_MAX && ((long long)a.rows * size < dev->sm_count || (a.vocab + size - 1) / size > 16384)) size *= 2;
+  while (size < CLUSTER_MAX && ((long long)a.rows * size < dev->sm_count || (a.vocab + size - 1) / size > (a.bf16 ? 32768 : 16384))) size *= 2;
   p.chunk = ((a.vocab + size - 1) / size + 15) / 16 * 16;
   p.seg = (p.chunk + THREADS - 1) / THREADS | 1;
   return a.bf16 ? launch<__nv_bfloat16>(dev, p, size) : launch<float>(dev, p, size);
