@@ -44,18 +44,27 @@ template <bool TREE> __device__ __forceinline__ bool check_sequence(const ugb_ma
 }
 
 // ------------------------------------------------------------- generic ------
-// grid (row tiles, key / value heads x sequences, slices), 256 threads as 16 x 16: rows ty * RM + i, keys tx + 16 j, columns 4 tx + 64 c.
-// Shared memory, all f32: queries [16 RM][dq + 4], keys and then values of a tile [64][max(dq, dv) + 4], probabilities [16 RM][64 + 4].
-// The products' operands come from shared memory four columns at a time (rows apart by an odd multiple of 16 bytes: no bank conflicts).
-template <typename T, int RM, int NC, bool TREE>
-__global__ void __launch_bounds__(256)
+// grid (row tiles, key / value heads x sequences, slices), 256 threads as 16 x 16: rows ty * RM + i, keys tx + 16 j, columns 4 tx + 64 c.  The keys
+// that the rows see form one list, without the gap between the first ones and the window, cut into tiles of 64.
+// Shared memory, all f32: queries [16 RM][dq + 4], keys [64][dq + 4], values [64][dv + 4], probabilities [16 RM][64 + 4].  The products' operands
+// come from there four columns at a time (rows apart by an odd multiple of 16 bytes: no bank conflicts).  COPIES: f32 rows that are aligned are copied
+// by cp.async, the keys of the next tile behind this one's scores, the values beside them.
+constexpr int KEYS = 64;
+__device__ __forceinline__ void copy16(float *dst, const float *src, bool valid) {      // zeros if not
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+template <typename T, int RM, int NC, bool TREE, bool COPIES>
+__global__ void __launch_bounds__(256, 2)
 masked_attention_generic_kernel(Params p) {
   constexpr int TR = 16 * RM, PLD = KEYS + 4;
   extern __shared__ __align__(16) float gsm[];
   __shared__ int up[TREE ? UGB_TREE_MAX : 1];
   __shared__ uint32_t bits[TREE ? TR * 4 : 1];             // of a row: which nodes its node sees
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, dq = p.dq, dv = p.dv, ld = max(dq, dv) + 4, qld = dq + 4;
-  float *qs = gsm, *ks = qs + TR * qld, *ps = ks + KEYS * ld;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, dq = p.dq, dv = p.dv, kld = dq + 4, vld = dv + 4;
+  float *qs = gsm, *ks = qs + TR * kld, *vs = ks + KEYS * kld, *ps = vs + KEYS * vld;
   const int s = blockIdx.y / p.kv_heads, kvh = blockIdx.y % p.kv_heads, row0 = blockIdx.x * TR, n_rows = min(TR, p.rows - row0);
   const int pos = p.mask.pos[s];
   if (!check_sequence<TREE>(p.mask, s, pos, up, p.status)) return;
@@ -69,13 +78,31 @@ masked_attention_generic_kernel(Params p) {
     }
   }
   const T *q = (const T *)p.q, *k = (const T *)p.k + ((size_t)s * p.kv_heads + kvh) * p.mask.t_max * dq, *v = (const T *)p.v + ((size_t)s * p.kv_heads + kvh) * p.mask.t_max * dv;
-  for (int i = threadIdx.x; i < TR * dq; i += 256) {
-    const int r = i / dq, c = i - r * dq, row = row0 + r;
-    qs[r * qld + c] = r < n_rows ? (float)q[(((size_t)s * p.mask.t + row / p.share) * p.heads + kvh * p.share + row % p.share) * dq + c] : 0.f;
-  }
   const int i0 = row0 / p.share, i1 = (row0 + n_rows - 1) / p.share;
   const Span span = span_of<TREE>(p.mask, pos, i0, i1);
-  const int per = (span.tiles + p.splits - 1) / p.splits, first = blockIdx.z * per, last = min(span.tiles, first + per);
+  const int n_keys = span.first + span.end - span.from, tiles = (n_keys + KEYS - 1) / KEYS;
+  const int per = (tiles + p.splits - 1) / p.splits, first = blockIdx.z * per, last = min(tiles, first + per);
+  auto key_of = [&](int at) { return at < span.first ? at : span.from + at - span.first; };      // position of a place in the list
+  // rows of 64 places of the list, 16 lanes a row
+  auto fetch = [&](const T *src, int d, float *dst, int ld, int tile) {
+    for (int r = ty; r < KEYS; r += 16) {
+      const int at = tile * KEYS + r;
+      const bool valid = at < n_keys;
+      const T *x = src + (size_t)(valid ? key_of(at) : 0) * d;
+      if constexpr (COPIES) {
+        for (int c = 4 * tx; c < d; c += 64) copy16(dst + r * ld + c, x + c, valid);
+      } else {
+        for (int c = tx; c < d; c += 16) dst[r * ld + c] = valid ? (float)x[c] : 0.f;
+      }
+    }
+    if constexpr (COPIES) copies_commit();
+  };
+  if (first < last) fetch(k, dq, ks, kld, first);
+  for (int r = ty; r < TR; r += 16) {
+    const int row = row0 + r;
+    const T *x = q + (((size_t)s * p.mask.t + row / p.share) * p.heads + kvh * p.share + row % p.share) * dq;
+    for (int c = tx; c < dq; c += 16) qs[r * kld + c] = r < n_rows ? (float)x[c] : 0.f;
+  }
   float m[RM], l[RM], o[RM][4 * NC];
   int at[RM];                                              // absolute position of a row's query
 #pragma unroll
@@ -87,13 +114,8 @@ masked_attention_generic_kernel(Params p) {
     for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
   }
   for (int tile = first; tile < last; ++tile) {
-    const int key0 = span.key0(tile);
-    auto seen = [&](int key) { return key < span.first || (key >= span.from && key < span.end); };      // by any row: the others may hold anything
-    __syncthreads();
-    for (int i = threadIdx.x; i < KEYS * dq; i += 256) {
-      const int key = i / dq, c = i - key * dq;
-      ks[key * ld + c] = seen(key0 + key) ? (float)k[(size_t)(key0 + key) * dq + c] : 0.f;
-    }
+    fetch(v, dv, vs, vld, tile);                           // its last readers are behind the barrier at the end of a tile
+    if constexpr (COPIES) copies_wait<1>();                // the keys
     __syncthreads();
     float sc[RM][4];
 #pragma unroll
@@ -103,9 +125,9 @@ masked_attention_generic_kernel(Params p) {
     for (int c = 0; c < dq; c += 4) {
       float4 a[RM], b[4];
 #pragma unroll
-      for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4 *>(qs + (ty * RM + i) * qld + c);
+      for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4 *>(qs + (ty * RM + i) * kld + c);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4 *>(ks + (tx + 16 * j) * ld + c);
+      for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4 *>(ks + (tx + 16 * j) * kld + c);
 #pragma unroll
       for (int i = 0; i < RM; ++i)
 #pragma unroll
@@ -121,7 +143,7 @@ masked_attention_generic_kernel(Params p) {
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int key = key0 + tx + 16 * j;
+        const int place = tile * KEYS + tx + 16 * j, key = key_of(place);
         bool on;
         if constexpr (TREE) {
           const int node = key - pos;
@@ -129,7 +151,7 @@ masked_attention_generic_kernel(Params p) {
         } else {
           on = key <= at[i] && (key > at[i] - p.mask.window || key < p.mask.sinks);
         }
-        sc[i][j] = on ? sc[i][j] * p.scale : -INFINITY;
+        sc[i][j] = on && place < n_keys ? sc[i][j] * p.scale : -INFINITY;
         mx = fmaxf(mx, sc[i][j]);
       }
 #pragma unroll
@@ -148,12 +170,9 @@ masked_attention_generic_kernel(Params p) {
 #pragma unroll
       for (int c = 0; c < 4 * NC; ++c) o[i][c] *= alpha;
     }
+    if constexpr (COPIES) copies_wait<0>();                // the values
     __syncthreads();
-    for (int i = threadIdx.x; i < KEYS * dv; i += 256) {
-      const int key = i / dv, c = i - key * dv;
-      ks[key * ld + c] = seen(key0 + key) ? (float)v[(size_t)(key0 + key) * dv + c] : 0.f;
-    }
-    __syncthreads();
+    if (tile + 1 < last) fetch(k, dq, ks, kld, tile + 1);  // the scores are done with the keys
     for (int key = 0; key < KEYS; key += 4) {
       float4 w[RM];
 #pragma unroll
@@ -163,7 +182,7 @@ masked_attention_generic_kernel(Params p) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           if (4 * tx + 64 * c >= dv) continue;
-          const float4 b = *reinterpret_cast<const float4 *>(ks + (key + e) * ld + 4 * tx + 64 * c);
+          const float4 b = *reinterpret_cast<const float4 *>(vs + (key + e) * vld + 4 * tx + 64 * c);
 #pragma unroll
           for (int i = 0; i < RM; ++i) {
             const float a = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
@@ -174,6 +193,7 @@ masked_attention_generic_kernel(Params p) {
           }
         }
     }
+    __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < RM; ++i) {
@@ -188,86 +208,88 @@ masked_attention_generic_kernel(Params p) {
       for (int c = 0; c < 4 * NC; ++c)
         if (4 * tx + 64 * (c / 4) < dv) out[4 * tx + 64 * (c / 4) + c % 4] = (T)(o[i][c] * f);
     } else {
-      const size_t slot = ((size_t)blockIdx.z * gridDim.y + blockIdx.y) * p.rows + row;
-      if (tx == 0) p.part_ml[slot] = make_float2(m[i], l[i]);
+      const size_t pair = (size_t)blockIdx.z * gridDim.y + blockIdx.y;
+      if (tx == 0) p.part_ml[pair * p.rows + row] = make_float2(m[i], l[i]);
 #pragma unroll
-      for (int c = 0; c < 4 * NC; ++c)
-        if (4 * tx + 64 * (c / 4) < dv) p.part_o[slot * dv + 4 * tx + 64 * (c / 4) + c % 4] = o[i][c];
+      for (int c = 0; c < NC; ++c)
+        if (4 * tx + 64 * c < dv) p.part_o[(pair * (dv / 4) + tx + 16 * c) * p.rows + row] = make_float4(o[i][4 * c], o[i][4 * c + 1], o[i][4 * c + 2], o[i][4 * c + 3]);
     }
   }
 }
 
 // ------------------------------------------------------------- combine ------
-// One warp per row: the slices in their order, whatever order they ran in.
+// One CTA per 32 rows of a pair: lane = row, warp = columns.  The slices in their order, whatever order they ran in.
 template <typename T, bool TREE>
 __global__ void __launch_bounds__(256)
 masked_combine_kernel(Params p, int pairs) {
-  const size_t n = (size_t)pairs * p.rows, at = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (at >= n) return;
-  const int pair = (int)(at / p.rows), row = (int)(at % p.rows), s = pair / p.kv_heads, kvh = pair % p.kv_heads, pos = p.mask.pos[s];
-  bool bad = pos < 0 || pos > p.mask.t_max - p.mask.t;
-  if constexpr (TREE)
-    for (int j = lane; j < p.mask.t; j += 32) {
-      const int a = p.mask.parents[(size_t)s * p.mask.t + j];
-      bad |= a < -1 || a >= j;
+  __shared__ float weight[UGB_MASKED_SPLITS][32], whole[32];
+  __shared__ T done[32][256 + 8];
+  __shared__ int up[TREE ? UGB_TREE_MAX : 1];
+  const int blocks = (p.rows + 31) / 32, pair = blockIdx.x / blocks, row0 = blockIdx.x % blocks * 32, n_rows = min(32, p.rows - row0);
+  const int s = pair / p.kv_heads, kvh = pair % p.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = row0 + min(lane, n_rows - 1);
+  if (!check_sequence<TREE>(p.mask, s, p.mask.pos[s], up, p.status)) return;     // nothing was computed
+  const size_t n = (size_t)pairs * p.rows, at = (size_t)pair * p.rows + row;
+  if (warp == 0) {
+    float m = -INFINITY, l = 0.f;
+    for (int z = 0; z < p.splits; ++z) m = fmaxf(m, p.part_ml[z * n + at].x);
+    for (int z = 0; z < p.splits; ++z) {
+      const float2 ml = p.part_ml[z * n + at];
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+      weight[z][lane] = f;
+      l = fmaf(f, ml.y, l);
     }
-  if (__any_sync(0xffffffffu, bad)) return;                // nothing was computed
-  float m = -INFINITY;
-  for (int z = lane; z < p.splits; z += 32) m = fmaxf(m, p.part_ml[(size_t)z * n + at].x);
-#pragma unroll
-  for (int e = 16; e > 0; e >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, e));
-  float l = 0.f;
-  for (int c0 = 0; c0 < p.dv; c0 += 128) {                 // dv is a multiple of 8
-    const int c = c0 + 4 * lane;
+    whole[lane] = l > 0.f ? p.out_scale / l : 0.f;
+  }
+  __syncthreads();
+  const float f = whole[lane];
+  for (int c = warp; c < p.dv / 4; c += 8) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    l = 0.f;
 #pragma unroll 4
     for (int z = 0; z < p.splits; ++z) {
-      const float2 ml = p.part_ml[(size_t)z * n + at];
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-      l = fmaf(f, ml.y, l);
-      if (c < p.dv && f > 0.f) {
-        const float4 v = *reinterpret_cast<const float4 *>(p.part_o + ((size_t)z * n + at) * p.dv + c);
-        acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
+      const float w = weight[z][lane];
+      if (w > 0.f) {                                       // what weighs nothing was not written either
+        const float4 v = p.part_o[(((size_t)z * pairs + pair) * (p.dv / 4) + c) * p.rows + row];
+        acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
       }
     }
-    const float f = l > 0.f ? p.out_scale / l : 0.f;
-    if (c < p.dv) {
-      T *out = (T *)p.out + (((size_t)s * p.mask.t + row / p.share) * p.heads + kvh * p.share + row % p.share) * p.dv + c;
-      out[0] = (T)(acc.x * f); out[1] = (T)(acc.y * f); out[2] = (T)(acc.z * f); out[3] = (T)(acc.w * f);
-    }
+    done[lane][4 * c] = (T)(acc.x * f); done[lane][4 * c + 1] = (T)(acc.y * f); done[lane][4 * c + 2] = (T)(acc.z * f); done[lane][4 * c + 3] = (T)(acc.w * f);
+  }
+  __syncthreads();
+  for (int r = warp; r < n_rows; r += 8) {
+    const int i = (row0 + r) / p.share, h = (row0 + r) % p.share;
+    T *out = (T *)p.out + (((size_t)s * p.mask.t + i) * p.heads + kvh * p.share + h) * p.dv;
+    for (int c = lane; c < p.dv; c += 32) out[c] = done[r][c];
   }
 }
 
-size_t generic_smem(int dq, int dv, int rows) { return (size_t)(rows * (dq + 4) + KEYS * (std::max(dq, dv) + 4) + rows * (KEYS + 4)) * 4; }
+size_t generic_smem(int dq, int dv, int rows) { return (size_t)((rows + KEYS) * (dq + 4) + KEYS * (dv + 4) + rows * (KEYS + 4)) * 4; }
 
-template <typename T, int RM, int NC, bool TREE> cudaError_t launch_generic(dim3 grid, size_t smem, cudaStream_t st, const Params &p) {
+template <typename T, int RM, int NC, bool TREE, bool COPIES> cudaError_t launch_generic(dim3 grid, size_t smem, cudaStream_t st, const Params &p) {
   static bool attr_set[64] = {};
   int ordinal = 0;
   cudaError_t e = cudaGetDevice(&ordinal);
   if (e != cudaSuccess) return e;
   if (!attr_set[ordinal & 63]) {
-    e = cudaFuncSetAttribute(masked_attention_generic_kernel<T, RM, NC, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)generic_smem(256, 256, 16 * RM));
+    e = cudaFuncSetAttribute(masked_attention_generic_kernel<T, RM, NC, TREE, COPIES>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)generic_smem(256, 256, 16 * RM));
     if (e != cudaSuccess) return e;
     attr_set[ordinal & 63] = true;
   }
-  masked_attention_generic_kernel<T, RM, NC, TREE><<<grid, 256, smem, st>>>(p);
+  masked_attention_generic_kernel<T, RM, NC, TREE, COPIES><<<grid, 256, smem, st>>>(p);
   return cudaSuccess;
 }
-template <typename T, int RM, bool TREE> cudaError_t launch_columns(dim3 grid, size_t smem, cudaStream_t st, const Params &p) {
-  if (p.dv <= 64) return launch_generic<T, RM, 1, TREE>(grid, smem, st, p);
-  if (p.dv <= 128) return launch_generic<T, RM, 2, TREE>(grid, smem, st, p);
-  return launch_generic<T, RM, 4, TREE>(grid, smem, st, p);
+template <typename T, int RM, bool TREE, bool COPIES> cudaError_t launch_columns(dim3 grid, size_t smem, cudaStream_t st, const Params &p) {
+  if (p.dv <= 64) return launch_generic<T, RM, 1, TREE, COPIES>(grid, smem, st, p);
+  if (p.dv <= 128) return launch_generic<T, RM, 2, TREE, COPIES>(grid, smem, st, p);
+  return launch_generic<T, RM, 4, TREE, COPIES>(grid, smem, st, p);
 }
-template <typename T> cudaError_t launch_rows(bool tree, int rm, dim3 grid, size_t smem, cudaStream_t st, const Params &p) {
-  if (rm == 1) return tree ? launch_columns<T, 1, true>(grid, smem, st, p) : launch_columns<T, 1, false>(grid, smem, st, p);
-  return tree ? launch_columns<T, 4, true>(grid, smem, st, p) : launch_columns<T, 4, false>(grid, smem, st, p);
+template <typename T, bool COPIES> cudaError_t launch_rows(bool tree, int rm, dim3 grid, size_t smem, cudaStream_t st, const Params &p) {
+  if (rm == 1) return tree ? launch_columns<T, 1, true, COPIES>(grid, smem, st, p) : launch_columns<T, 1, false, COPIES>(grid, smem, st, p);
+  return tree ? launch_columns<T, 4, true, COPIES>(grid, smem, st, p) : launch_columns<T, 4, false, COPIES>(grid, smem, st, p);
 }
 
 // Slices of the keys: as many as bring the CTAs to `slots`, of at least two tiles each (a slice costs a round of sums through memory).
 int slices(long long ctas, long long slots, int tiles) {
-  return (int)std::max(1LL, std::min({slots / std::max(1LL, ctas), (long long)(tiles + 1) / 2, 64LL}));
+  return (int)std::max(1LL, std::min({slots / std::max(1LL, ctas), (long long)(tiles + 1) / 2, (long long)UGB_MASKED_SPLITS}));
 }
 
 }  // namespace
@@ -292,8 +314,8 @@ int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a
   void *work = nullptr;
   if (p.splits > 1) {
     UGB_CUDA(dev, ugb_malloc_async(dev, &work, (size_t)p.splits * n * (size_t)(a.dv + 2) * 4));
-    p.part_o = (float *)work;
-    p.part_ml = (float2 *)(p.part_o + (size_t)p.splits * n * a.dv);
+    p.part_o = (float4 *)work;
+    p.part_ml = (float2 *)((float *)work + (size_t)p.splits * n * a.dv);
   }
   int32_t rc;
   if (tc) {
@@ -301,12 +323,14 @@ int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a
   } else {
     const size_t smem = generic_smem(a.dq, a.dv, 16 * rm);
     const dim3 grid((unsigned)row_tiles, (unsigned)pairs, (unsigned)p.splits);
-    const cudaError_t e = a.f32 ? launch_rows<float>(tree, rm, grid, smem, dev->stream, p) : launch_rows<__nv_bfloat16>(tree, rm, grid, smem, dev->stream, p);
+    const bool aligned = (((uintptr_t)a.k | (uintptr_t)a.v) & 15) == 0;
+    const cudaError_t e = !a.f32 ? launch_rows<__nv_bfloat16, false>(tree, rm, grid, smem, dev->stream, p)
+                          : aligned ? launch_rows<float, true>(tree, rm, grid, smem, dev->stream, p) : launch_rows<float, false>(tree, rm, grid, smem, dev->stream, p);
     rc = e != cudaSuccess ? ugb_fail(dev, UGB_ERR_CUDA, "launch of masked_attention_generic_kernel failed: %s", cudaGetErrorString(e))
                           : ugb_after_launch(dev, "masked_attention_generic_kernel");
   }
   if (rc == UGB_OK && p.splits > 1) {
-    const dim3 rows((unsigned)((n + 7) / 8));
+    const dim3 rows((unsigned)(pairs * ((p.rows + 31) / 32)));
     if (a.f32) tree ? masked_combine_kernel<float, true><<<rows, 256, 0, dev->stream>>>(p, pairs) : masked_combine_kernel<float, false><<<rows, 256, 0, dev->stream>>>(p, pairs);
     else tree ? masked_combine_kernel<__nv_bfloat16, true><<<rows, 256, 0, dev->stream>>>(p, pairs) : masked_combine_kernel<__nv_bfloat16, false><<<rows, 256, 0, dev->stream>>>(p, pairs);
     rc = ugb_after_launch(dev, "masked_combine_kernel");

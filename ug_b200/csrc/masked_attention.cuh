@@ -21,32 +21,28 @@ struct ugb_mask {
   const int *pos, *parents;
   int t, t_max, sinks, window;
 };
+constexpr int UGB_MASKED_SPLITS = 64;    // slices of the keys, at most
 struct ugb_masked_params {
   const void *q, *k, *v;
   void *out;
   ugb_mask mask;
   int heads, kv_heads, share, rows, dq, dv, splits;        // rows: t * share, of a sequence and key / value head
   float scale, out_scale;                                  // scale: with log2(e)
-  float *part_o;                                           // of slices: [splits][b][kv_heads][rows][dv]
-  float2 *part_ml;                                         // (maximum, sum) alike
+  float4 *part_o;                                          // of slices: [splits][b][kv_heads][dv / 4][rows], so that threads of neighbouring rows
+                                                           // write and read neighbouring pieces
+  float2 *part_ml;                                         // (maximum, sum) [splits][b][kv_heads][rows]
   ugb_status_word *status;
 };
 
 #ifdef __CUDACC__
 namespace ugb_masked {
 
-constexpr int KEYS = 64;     // of a tile
-
 __device__ __forceinline__ void raise_invalid(ugb_status_word *status, int detail) {
   if (atomicCAS(&status->code, 0u, (unsigned)UGB_ERR_INVALID) == 0u) status->detail = (unsigned)detail;
 }
 
-// The keys that rows of queries i0 .. i1 of a sequence see: positions below `first` and from `from` on, up to `end` - 1, in tiles of KEYS
-// positions that start at multiples of KEYS.
-struct Span {
-  int first, from, end, first_tiles, from_tile, tiles;
-  __device__ __forceinline__ int key0(int tile) const { return (tile < first_tiles ? tile : from_tile + tile - first_tiles) * KEYS; }
-};
+// The keys that rows of queries i0 .. i1 of a sequence see: positions below `first`, and from `from` to `end` - 1.
+struct Span { int first, from, end; };
 template <bool TREE> __device__ __forceinline__ Span span_of(const ugb_mask &m, int pos, int i0, int i1) {
   Span s;
   s.end = pos + i1 + 1;
@@ -56,9 +52,6 @@ template <bool TREE> __device__ __forceinline__ Span span_of(const ugb_mask &m, 
     s.from = max(0, pos + i0 - m.window + 1);
     s.first = min(m.sinks, s.from);
   }
-  s.first_tiles = (s.first + KEYS - 1) / KEYS;
-  s.from_tile = max(s.from / KEYS, s.first_tiles);
-  s.tiles = s.first_tiles + max(0, (s.end + KEYS - 1) / KEYS - s.from_tile);
   return s;
 }
 

@@ -1,15 +1,19 @@
 // Attention over a window or a tree on the 5th-generation tensor cores (see masked_attention.cuh), bf16 heads of 64 or 128 values.
 //
-// One item = up to RT x 128 rows of a (sequence, key / value head) and a slice of the keys they see, in tiles of 64 keys; a row is a query
-// position of one head of the group, so that keys and values are read once for all heads that share them:
-//     warp 0        TMA producer: the rows' queries (one box: heads x positions), then key and value tiles into rings
-//     warp 1        MMA issuer:   S = Q K^T of each 128 rows into one of two TMEM buffers, O += P V, accumulated in TMEM
+// One item = up to RT x 128 rows of a (sequence, key / value head) and a slice of the keys they see, in tiles of 128 keys (64 where 64 are enough); a row is
+// a query position of one head of the group, so that keys and values are read once for all heads that share them:
+//     warp 0        TMA producer: the rows' queries (one box: heads x positions), then key and value tiles into a ring
+//     warp 1        MMA issuer:   S = Q K^T of each 128 rows, O += P V, both accumulated in TMEM
 //     then 4 warps  softmax of 128 rows each (RT groups): one row per thread, no shuffles; P in bf16 through shared memory
-// While one group's softmax runs, the other's products do.  O stays in TMEM from the first tile to the last: it is rescaled only where a row's
-// maximum has grown by more than 2^8 since it was last (the probabilities are then up to 2^8, which costs bf16 no precision, and the sum is f32), which
-// after the first tiles is hardly ever.  Rows of V that no row of the item sees are set to zero in shared memory: P is zero there, but 0 x NaN is not.
+// The scores of the next tile are formed as soon as this tile's are in registers, so that the softmax finds them ready; while one group's softmax runs, the
+// other's products do.  O stays in TMEM from the first tile to the last: it is rescaled only where a row's maximum has grown by more than 2^8 since
+// it was last (the probabilities are then up to 2^8, which costs bf16 no precision, and the sum is f32), which after the first tiles is hardly ever.
+// Results leave through shared memory, by TMA.  Rows of V that no row of the item sees are set to zero there: P is zero for them, but 0 x NaN is not.
 // Grid: one CTA per item; a CTA that is done takes over the item of one that has not started (cluster launch control), so that its set-up and its
 // TMEM are shared by many and long and short items even out.  Every wait on an mbarrier is bounded.
+//
+// Tiles of 128 keys and not 64: the waits, fences and stores of a tile cost a softmax warp 1000 cycles whatever its size, the exponentials of 64 keys
+// 950 to 1600; and the products read Q and P from shared memory once per 128 keys.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -24,23 +28,24 @@ using namespace ugb_tc;
 using namespace ugb_masked;
 
 constexpr int BQ = 128, CB = 64;                           // rows of a group, columns of a block (one 128-byte swizzle row)
-constexpr int P_BYTES = BQ * KEYS * 2, Q_BLOCK = BQ * CB * 2, KV_BLOCK = KEYS * CB * 2;
-static_assert(KEYS == 64, "one 128-byte swizzle row of probabilities, one 64-bit mask");
+constexpr int KEYS = 128;                                  // of a tile
+constexpr int BLOCK = 128 * CB * 2;                        // 128 rows of 64 columns: 16 KiB
+constexpr int P_BYTES = 2 * BLOCK;                         // 128 rows x 128 keys
 
 template <int DQ, int DV, int RT> struct Shape {
   static constexpr int THREADS = 64 + 128 * RT;
-  static constexpr int Q_BYTES = BQ * DQ * 2, K_BYTES = KEYS * DQ * 2, V_BYTES = KEYS * DV * 2;
-  static constexpr int O_COL = RT * 2 * KEYS;              // TMEM: S [RT][2][64], then O [RT][DV]
+  static constexpr int Q_BYTES = DQ / CB * BLOCK, STAGE = (DQ > DV ? DQ : DV) / CB * BLOCK;     // a stage holds a tile of keys or of values
+  static constexpr int O_COL = RT * KEYS;                  // TMEM: S [RT][128], then O [RT][DV]
   static constexpr int TMEM_USED = O_COL + RT * DV, TMEM_COLS = TMEM_USED <= 256 ? 256 : 512;
   static constexpr int FIXED = RT * (Q_BYTES + P_BYTES) + 1024 /*alignment*/ + 512 /*barriers*/;
   // one group of 64-wide heads: two CTAs per SM, since one softmax warp per tile does not keep up with HBM
   static constexpr int CTAS_PER_SM = RT == 1 && DQ + DV == 128 ? 2 : 1;
-  static constexpr int LIMIT = CTAS_PER_SM == 2 ? 112 * 1024 : 224 * 1024;
-  static constexpr int FIT = (LIMIT - FIXED) / (K_BYTES + V_BYTES), STAGES = FIT > 8 ? 8 : FIT;
-  static constexpr int TILES = FIXED + STAGES * (K_BYTES + V_BYTES);
+  static constexpr int LIMIT = CTAS_PER_SM == 2 ? 112 * 1024 : 225 * 1024 + 512;
+  static constexpr int FIT = (LIMIT - FIXED) / STAGE, STAGES = FIT > 8 ? 8 : FIT;
+  static constexpr int TILES = FIXED + STAGES * STAGE;
   // a CTA that takes all of the TMEM is alone on its SM: more than half of the shared memory sees to that
   static constexpr int SMEM_BYTES = CTAS_PER_SM == 1 && TILES < 116 * 1024 ? 116 * 1024 : TILES;
-  static_assert(TMEM_USED <= 512 && STAGES >= 2 && SMEM_BYTES <= 227 * 1024, "tile shape");
+  static_assert(TMEM_USED <= 512 && STAGES >= 3 && SMEM_BYTES <= 226 * 1024, "tile shape");
 };
 
 struct Params {
@@ -88,14 +93,27 @@ __device__ __forceinline__ bool group_or(int id, bool v) {
                : "=r"(r) : "r"((uint32_t)v), "r"(id) : "memory");
   return r != 0;
 }
+__device__ __forceinline__ void group_sync(int id) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap *map, uint32_t src, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 // The lowest n bits, n clamped to 0 .. 64.
 __device__ __forceinline__ unsigned long long low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
 // Items in the order of their block index: the last rows of every pair first (they see the most keys), their slices side by side.
 struct Item {
   int s, kvh, slice, row0, pos, first, tiles;              // first: of the slice's tiles; tiles: 0 = nothing to compute
+  int first_tiles, start;                                  // tiles of the first positions; where the others start
   bool valid;                                              // the sequence exists and its position is inside the cache
   Span span;
+  // tile j of the slice: its first key, and whether it has more than 64
+  __device__ __forceinline__ int key0(int j) const { return first + j < first_tiles ? (first + j) * KEYS : start + (first + j - first_tiles) * KEYS; }
+  __device__ __forceinline__ bool full(int j) const {      // the last of the first tiles may hold the start of the window too
+    return (first + j < first_tiles && span.from >= first_tiles * KEYS ? span.first : span.end) - key0(j) > 64;
+  }
 };
 template <int RT, bool TREE> __device__ __forceinline__ Item item_of(int idx, const Params &p) {
   Item it;
@@ -110,29 +128,33 @@ template <int RT, bool TREE> __device__ __forceinline__ Item item_of(int idx, co
   if (it.valid) {
     const int last = min(it.row0 + RT * p.per_group, p.m.rows) - 1;
     it.span = span_of<TREE>(p.m.mask, it.pos, it.row0 / p.m.share, last / p.m.share);
-    const int per = (it.span.tiles + p.m.splits - 1) / p.m.splits;
+    it.first_tiles = (it.span.first + KEYS - 1) / KEYS;
+    it.start = max(it.span.from, it.first_tiles * KEYS);
+    const int tiles = it.first_tiles + max(0, it.span.end - it.start + KEYS - 1) / KEYS;
+    const int per = (tiles + p.m.splits - 1) / p.m.splits;
     it.first = it.slice * per;
-    it.tiles = max(0, min(it.span.tiles, it.first + per) - it.first);
+    it.tiles = max(0, min(tiles, it.first + per) - it.first);
   }
   return it;
 }
 
 template <int DQ, int DV, int RT, bool TREE>
 __global__ void __launch_bounds__((Shape<DQ, DV, RT>::THREADS), (Shape<DQ, DV, RT>::CTAS_PER_SM))
-masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, Params p) {
+masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                           const __grid_constant__ CUtensorMap tmO, Params p) {
   using Sh = Shape<DQ, DV, RT>;
   constexpr int ST = Sh::STAGES;
   extern __shared__ uint8_t smem_raw[];
   __shared__ int up[TREE ? RT : 1][TREE ? UGB_TREE_MAX : 1];
   uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t *q_s = smem, *p_s = q_s + RT * Sh::Q_BYTES, *k_s = p_s + RT * P_BYTES, *v_s = k_s + ST * Sh::K_BYTES;
-  uint64_t *bars = (uint64_t *)(v_s + ST * Sh::V_BYTES);
+  uint8_t *q_s = smem, *p_s = q_s + RT * Sh::Q_BYTES, *kv_s = p_s + RT * P_BYTES;
+  uint64_t *bars = (uint64_t *)(kv_s + ST * Sh::STAGE);
   uint64_t *q_full = bars, *q_empty = bars + 1, *answer_full = bars + 2, *answer = bars + 4;       // the answer: 16 bytes, aligned
-  uint64_t *item_full = bars + 6, *item_empty = bars + 8, *s_full = bars + 10, *p_full = s_full + 2 * RT, *o_full = p_full + RT;
-  uint64_t *k_full = o_full + RT, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST;
-  uint32_t *tmem_slot = (uint32_t *)(v_empty + ST);
+  uint64_t *item_full = bars + 6, *item_empty = bars + 8, *s_full = bars + 10, *s_free = s_full + RT, *p_full = s_free + RT, *o_full = p_full + RT;
+  uint64_t *kv_full = o_full + RT, *kv_empty = kv_full + ST;
+  uint32_t *tmem_slot = (uint32_t *)(kv_empty + ST);
   volatile int *abort_flag = (volatile int *)(tmem_slot + 1), *item_slot = (volatile int *)(tmem_slot + 2);      // two entries
-  static_assert((10 + 4 * RT + 4 * ST) * 8 + 16 <= 512, "barriers fit");
+  static_assert((10 + 4 * RT + 2 * ST) * 8 + 16 <= 512, "barriers fit");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ugb_status_word *const status = p.m.status;
@@ -144,22 +166,22 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
       mbar_init(smem_u32(&item_full[i]), 1);
       mbar_init(smem_u32(&item_empty[i]), 1 + 4 * RT);
     }
-    for (int i = 0; i < 2 * RT; ++i) mbar_init(smem_u32(&s_full[i]), 1);
     for (int i = 0; i < RT; ++i) {
+      mbar_init(smem_u32(&s_full[i]), 1);
+      mbar_init(smem_u32(&s_free[i]), 4);
       mbar_init(smem_u32(&p_full[i]), 4);
       mbar_init(smem_u32(&o_full[i]), 1);
     }
     for (int i = 0; i < ST; ++i) {
-      mbar_init(smem_u32(&k_full[i]), 1);
-      mbar_init(smem_u32(&k_empty[i]), 1);
-      mbar_init(smem_u32(&v_full[i]), 1);
-      mbar_init(smem_u32(&v_empty[i]), 1);
+      mbar_init(smem_u32(&kv_full[i]), 1);
+      mbar_init(smem_u32(&kv_empty[i]), 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmQ) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmK) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmV) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&tmO) : "memory");
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(Sh::TMEM_COLS) : "memory");
@@ -170,10 +192,11 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // The ring's order: K(0), then K(j + 1), V(j) for every tile j, and V of the last one: the order in which the products are issued.
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer --
     if (elect_one()) {
-      int g = 0, n_q = 0, idx = blockIdx.x;                // tiles and items with tiles so far
+      int g = 0, n_q = 0, idx = blockIdx.x;                // stages filled and items with tiles so far
       for (int n_it = 0;; ++n_it) {
         const int at = n_it & 1;
         if (!mbar_wait(smem_u32(&item_empty[at]), ((uint32_t)(n_it >> 1) & 1u) ^ 1u, abort_flag, status, 0x60)) break;
@@ -185,28 +208,30 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
         next_item_request(smem_u32(answer), smem_u32(answer_full));
         const Item it = item_of<RT, TREE>(idx, p);
         bool alive = true;
+        auto load = [&](const CUtensorMap *map, int d, int j) {          // tile j of the keys or values
+          const int s = g % ST, n = it.full(j) ? 2 : 1, key0 = it.key0(j);
+          if (!mbar_wait(smem_u32(&kv_empty[s]), ((uint32_t)(g / ST) & 1u) ^ 1u, abort_flag, status, 0x61)) { alive = false; return; }
+          ++g;
+          mbar_expect_tx(smem_u32(&kv_full[s]), (uint32_t)(n * 64 * d * 2));
+          for (int c = 0; c < d / CB; ++c)
+            for (int h = 0; h < n; ++h)
+              tma_load_4d(smem_u32(kv_s + s * Sh::STAGE + c * BLOCK + h * (BLOCK / 2)), map, smem_u32(&kv_full[s]), c * CB, it.kvh, key0 + 64 * h, it.s);
+        };
         if (it.tiles > 0) {
           const int i0 = it.row0 / p.m.share, step = p.per_group / p.m.share;
           // the query buffers are free once every S product of the item before has retired
-          alive = mbar_wait(smem_u32(q_empty), ((uint32_t)n_q & 1u) ^ 1u, abort_flag, status, 0x61);
+          alive = mbar_wait(smem_u32(q_empty), ((uint32_t)n_q & 1u) ^ 1u, abort_flag, status, 0x62);
           ++n_q;
           if (alive) {
             mbar_expect_tx(smem_u32(q_full), (uint32_t)(RT * (DQ / CB) * p.per_group * CB * 2));
             for (int a = 0; a < RT; ++a)
               for (int c = 0; c < DQ / CB; ++c)
-                tma_load_4d(smem_u32(q_s + a * Sh::Q_BYTES + c * Q_BLOCK), &tmQ, smem_u32(q_full), c * CB, it.kvh * p.m.share, i0 + a * step, it.s);
+                tma_load_4d(smem_u32(q_s + a * Sh::Q_BYTES + c * BLOCK), &tmQ, smem_u32(q_full), c * CB, it.kvh * p.m.share, i0 + a * step, it.s);
+            load(&tmK, DQ, 0);
           }
-          for (int j = 0; j < it.tiles && alive; ++j, ++g) {
-            const int s = g % ST, key0 = it.span.key0(it.first + j);
-            const uint32_t ph = (uint32_t)(g / ST) & 1u;
-            if (!mbar_wait(smem_u32(&k_empty[s]), ph ^ 1u, abort_flag, status, 0x62)) { alive = false; break; }
-            mbar_expect_tx(smem_u32(&k_full[s]), Sh::K_BYTES);
-            for (int c = 0; c < DQ / CB; ++c)
-              tma_load_4d(smem_u32(k_s + s * Sh::K_BYTES + c * KV_BLOCK), &tmK, smem_u32(&k_full[s]), c * CB, it.kvh, key0, it.s);
-            if (!mbar_wait(smem_u32(&v_empty[s]), ph ^ 1u, abort_flag, status, 0x63)) { alive = false; break; }
-            mbar_expect_tx(smem_u32(&v_full[s]), Sh::V_BYTES);
-            for (int c = 0; c < DV / CB; ++c)
-              tma_load_4d(smem_u32(v_s + s * Sh::V_BYTES + c * KV_BLOCK), &tmV, smem_u32(&v_full[s]), c * CB, it.kvh, key0, it.s);
+          for (int j = 0; j < it.tiles && alive; ++j) {
+            if (j + 1 < it.tiles) load(&tmK, DQ, j + 1);
+            if (alive) load(&tmV, DV, j);
           }
         }
         if (!mbar_wait(smem_u32(answer_full), (uint32_t)n_it & 1u, abort_flag, status, 0x64)) break;
@@ -218,11 +243,13 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer --
     if (elect_one()) {
-      const uint32_t idesc_s = make_idesc(BQ, KEYS, false);             // Q and K both K-major
-      const uint32_t idesc_o = make_idesc(BQ, DV, true);                // P K-major, V MN-major ([key][dim] rows)
-      bool alive = true;
-      int g0 = 0, n_q = 0, n_s[RT] = {}, n_p[RT] = {};                  // tiles, items, S and P V products so far
-      for (int n_it = 0; alive; ++n_it) {
+      // Q and K both K-major; P K-major, V MN-major ([key][dim] rows, blocks of 64 columns BLOCK apart)
+      const uint32_t idesc_s[2] = {make_idesc(BQ, 64, false), make_idesc(BQ, 128, false)}, idesc_o = make_idesc(BQ, DV, true);
+      const uint64_t q_desc = make_smem_desc(smem_u32(q_s), 0, 1024), p_desc = make_smem_desc(smem_u32(p_s), 0, 1024);
+      const uint64_t k_desc = make_smem_desc(smem_u32(kv_s), 0, 1024), v_desc = make_smem_desc(smem_u32(kv_s), BLOCK, 1024);
+      int g = 0, n_q = 0;                                               // stages and items so far
+      uint32_t n_s[2] = {0, 0}, n_p[2] = {0, 0};                        // S and P V products of a group so far
+      for (int n_it = 0;; ++n_it) {
         const int at = n_it & 1;
         if (!mbar_wait(smem_u32(&item_full[at]), (uint32_t)(n_it >> 1) & 1u, abort_flag, status, 0x65)) break;
         const int idx = item_slot[at];
@@ -232,56 +259,73 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
         if (it.tiles == 0) continue;
         if (!mbar_wait(smem_u32(q_full), (uint32_t)n_q & 1u, abort_flag, status, 0x66)) break;
         ++n_q;
-        const int groups = RT == 1 || it.row0 + p.per_group >= p.m.rows ? 1 : RT;
-        auto issue_s = [&](int j, int a) {                              // S of tile j, group a
-          const int s = (g0 + j) % ST;
-          if (a == 0 && !mbar_wait(smem_u32(&k_full[s]), (uint32_t)((g0 + j) / ST) & 1u, abort_flag, status, 0x67)) { alive = false; return; }
-          tcgen05_fence_after();
-          const int buf = n_s[a]++ & 1;
-          const uint32_t qa = smem_u32(q_s + a * Sh::Q_BYTES), kb = smem_u32(k_s + s * Sh::K_BYTES);
+        const bool both = RT == 2 && it.row0 + p.per_group < p.m.rows;
+        bool alive = true;
+        auto scores = [&](int j) {                                      // S of tile j, of every group
+          const int s = g % ST;
+          if (!mbar_wait(smem_u32(&kv_full[s]), (uint32_t)(g / ST) & 1u, abort_flag, status, 0x67)) { alive = false; return; }
+          ++g;
+          const uint64_t kd = k_desc + (uint64_t)(s * (Sh::STAGE >> 4));
+          const uint32_t idesc = idesc_s[it.full(j) ? 1 : 0];
 #pragma unroll
-          for (int kk = 0; kk < DQ / UMMA_K; ++kk)
-            umma_bf16(tmem + (uint32_t)((a * 2 + buf) * KEYS), make_smem_desc(qa + (kk / 4) * Q_BLOCK + (kk % 4) * (UMMA_K * 2), 0, 1024),
-                      make_smem_desc(kb + (kk / 4) * KV_BLOCK + (kk % 4) * (UMMA_K * 2), 0, 1024), idesc_s, kk > 0 ? 1u : 0u);
-          if (a == groups - 1) {
-            umma_commit(smem_u32(&k_empty[s]));
-            if (j == it.tiles - 1) umma_commit(smem_u32(q_empty));      // no more products read the queries
-          }
-          umma_commit(smem_u32(&s_full[a * 2 + buf]));
-        };
-        for (int j = 0; j < 2 && j < it.tiles; ++j)
-          for (int a = 0; a < groups && alive; ++a) issue_s(j, a);
-        for (int j = 0; j < it.tiles && alive; ++j) {
-          const int s = (g0 + j) % ST;
-          for (int a = 0; a < groups && alive; ++a) {
-            if (!mbar_wait(smem_u32(&p_full[a]), (uint32_t)n_p[a] & 1u, abort_flag, status, 0x68)) { alive = false; break; }
-            ++n_p[a];
-            if (a == 0 && !mbar_wait(smem_u32(&v_full[s]), (uint32_t)((g0 + j) / ST) & 1u, abort_flag, status, 0x69)) { alive = false; break; }
+          for (int a = 0; a < RT; ++a) {
+            if (a == 1 && !both) break;
+            // the group has taken the scores before out of the tensor memory
+            if (!mbar_wait(smem_u32(&s_free[a]), (n_s[a] & 1u) ^ 1u, abort_flag, status, 0x68)) { alive = false; return; }
+            ++n_s[a];
             tcgen05_fence_after();
-            const uint32_t pa = smem_u32(p_s + a * P_BYTES), vb = smem_u32(v_s + s * Sh::V_BYTES);
+            const uint64_t qd = q_desc + (uint64_t)(a * (Sh::Q_BYTES >> 4));
 #pragma unroll
-            for (int kk = 0; kk < KEYS / UMMA_K; ++kk)
-              umma_bf16(tmem + (uint32_t)(Sh::O_COL + a * DV), make_smem_desc(pa + kk * (UMMA_K * 2), 0, 1024),
-                        make_smem_desc(vb + kk * (UMMA_K * 128), KEYS * 128, 1024), idesc_o, j > 0 || kk > 0 ? 1u : 0u);
-            if (a == groups - 1) umma_commit(smem_u32(&v_empty[s]));
-            umma_commit(smem_u32(&o_full[a]));
-            // the score buffer of tile j + 2 is the one that the softmax released before this product could be issued
-            if (j + 2 < it.tiles) issue_s(j + 2, a);
+            for (int kk = 0; kk < DQ / UMMA_K; ++kk) {                  // 16 columns are 32 bytes inside the swizzled row
+              const uint64_t off = (uint64_t)(((kk / 4) * BLOCK + (kk % 4) * (UMMA_K * 2)) >> 4);
+              umma_bf16(tmem + (uint32_t)(a * KEYS), qd + off, kd + off, idesc, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(smem_u32(&s_full[a]));
           }
+          umma_commit(smem_u32(&kv_empty[s]));
+          if (j == it.tiles - 1) umma_commit(smem_u32(q_empty));        // no more products read the queries
+        };
+        scores(0);
+        for (int j = 0; j < it.tiles && alive; ++j) {
+          if (j + 1 < it.tiles) scores(j + 1);
+          if (!alive) break;
+          const int s = g % ST;
+          if (!mbar_wait(smem_u32(&kv_full[s]), (uint32_t)(g / ST) & 1u, abort_flag, status, 0x69)) { alive = false; break; }
+          ++g;
+          const uint64_t vd = v_desc + (uint64_t)(s * (Sh::STAGE >> 4));
+          const bool full = it.full(j);
+#pragma unroll
+          for (int a = 0; a < RT; ++a) {
+            if (a == 1 && !both) break;
+            if (!mbar_wait(smem_u32(&p_full[a]), n_p[a] & 1u, abort_flag, status, 0x6a)) { alive = false; break; }
+            ++n_p[a];
+            tcgen05_fence_after();
+            const uint64_t pd = p_desc + (uint64_t)(a * (P_BYTES >> 4));
+#pragma unroll
+            for (int kk = 0; kk < KEYS / UMMA_K; ++kk) {
+              if (kk >= 4 && !full) break;
+              // P: 16 keys are 32 bytes inside the swizzled row, 64 keys a block; V: 16 keys are 16 rows
+              umma_bf16(tmem + (uint32_t)(Sh::O_COL + a * DV), pd + (uint64_t)(((kk / 4) * BLOCK + (kk % 4) * (UMMA_K * 2)) >> 4),
+                        vd + (uint64_t)((kk * (UMMA_K * 128)) >> 4), idesc_o, j > 0 || kk > 0 ? 1u : 0u);
+            }
+            umma_commit(smem_u32(&o_full[a]));
+          }
+          if (alive) umma_commit(smem_u32(&kv_empty[s]));
         }
-        g0 += it.tiles;
+        if (!alive) break;
       }
     }
   } else {
     // -------------------------------------------------------------- softmax warps --
     const int a = (warp - 2) / 4, quad = warp & 3, row = quad * 32 + lane;              // TMEM lane = row of the group
-    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16), o_base = lane_base + (uint32_t)(Sh::O_COL + a * DV);
-    uint8_t *const prow = p_s + a * P_BYTES + row * 128;
-    bool alive = true;
-    int g0 = 0, n_s = 0, n_o = 0;                          // tiles of the CTA; S and O products of this group so far
-    for (int n_it = 0; alive; ++n_it) {
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16), s_base = lane_base + (uint32_t)(a * KEYS), o_base = lane_base + (uint32_t)(Sh::O_COL + a * DV);
+    uint8_t *const p_group = p_s + a * P_BYTES, *const prow = p_group + row * 128;
+    const bool leader = threadIdx.x == 64 + a * 128;       // issues the group's stores
+    int g0 = 0;                                            // stages of the CTA so far
+    uint32_t n_s = 0, n_o = 0;                             // S and O products of this group so far
+    for (int n_it = 0;; ++n_it) {
       const int at = n_it & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&item_full[at]), (uint32_t)(n_it >> 1) & 1u, abort_flag, status, 0x6a))) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&item_full[at]), (uint32_t)(n_it >> 1) & 1u, abort_flag, status, 0x6b))) break;
       const int idx = item_slot[at];
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&item_empty[at]));
@@ -292,7 +336,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
         continue;
       }
       const int r0 = it.row0 + a * p.per_group, n_rows = min(p.per_group, p.m.rows - r0);      // of this group
-      if (n_rows <= 0) { g0 += it.tiles; continue; }
+      if (n_rows <= 0) { g0 += 2 * it.tiles; continue; }
       const bool mine = row < n_rows;                      // this thread has a row
       const bool busy = quad * 32 < n_rows;                // this warp has rows
       const int i = (r0 + min(row, n_rows - 1)) / p.m.share, n = it.pos + i;
@@ -311,99 +355,119 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
             for (int j = i; j >= 0; j = up[a][j]) (j < 64 ? nodes0 : nodes1) |= 1ull << (j & 63);
         }
       }
+      // which of the 64 keys from key0 on this row sees
+      auto seen_from = [&](int key0) -> unsigned long long {
+        if constexpr (TREE) {
+          const int rel = key0 - it.pos;                   // node of the first key
+          if (rel <= -64) return ~0ull;
+          if (rel < 0) return (nodes0 << -rel) | low_bits(-rel);
+          if (rel < 64) return (nodes0 >> rel) | (rel ? nodes1 << (64 - rel) : 0ull);
+          return rel < 128 ? nodes1 >> (rel - 64) : 0ull;
+        } else {
+          return low_bits(n - key0 + 1) & (~low_bits(n - p.m.mask.window - key0 + 1) | low_bits(p.m.mask.sinks - key0));
+        }
+      };
       const float sc = p.m.scale;
       float m_ref = -INFINITY, l = 0.f;
+      bool alive = true;
       for (int j = 0; j < it.tiles; ++j) {
-        const int key0 = it.span.key0(it.first + j);
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[a * 2 + (n_s & 1)]), (uint32_t)(n_s >> 1) & 1u, abort_flag, status, 0x6b))) { alive = false; break; }
-        const int buf = n_s & 1;
+        const int key0 = it.key0(j);
+        const bool full = it.full(j);
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[a]), n_s & 1u, abort_flag, status, 0x6c))) { alive = false; break; }
         ++n_s;
-        uint32_t w[32];
-        float alpha = 1.f;
-        bool grow = false;
         if (busy) {
           tcgen05_fence_after();
-          float f[64];
+          uint32_t f[KEYS];                                // scores, and in their place, two to a register, the probabilities
           {
-            uint32_t r0_[32], r1_[32];
-            tmem_ld_32x32b_x32(lane_base + (uint32_t)((a * 2 + buf) * KEYS), r0_);
-            tmem_ld_32x32b_x32(lane_base + (uint32_t)((a * 2 + buf) * KEYS + 32), r1_);
-            tmem_ld_wait();
+            uint32_t(*r)[32] = reinterpret_cast<uint32_t(*)[32]>(f);    // what a half tile leaves in the upper columns is replaced below
 #pragma unroll
-            for (int e = 0; e < 32; ++e) { f[e] = __uint_as_float(r0_[e]); f[32 + e] = __uint_as_float(r1_[e]); }
+            for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_base + 32 * c, r[c]);
           }
-          unsigned long long seen;
-          if constexpr (TREE) {
-            const int rel = key0 - it.pos;                 // node of the tile's first key
-            if (rel <= -64) seen = ~0ull;
-            else if (rel < 0) seen = (nodes0 << -rel) | low_bits(-rel);
-            else if (rel < 64) seen = (nodes0 >> rel) | (rel ? nodes1 << (64 - rel) : 0ull);
-            else seen = rel < 128 ? nodes1 >> (rel - 64) : 0ull;
-          } else {
-            seen = low_bits(n - key0 + 1) & (~low_bits(n - p.m.mask.window - key0 + 1) | low_bits(p.m.mask.sinks - key0));
-          }
-          if (__any_sync(0xffffffffu, seen != ~0ull)) {
-            const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
+          tmem_ld_wait();
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&s_free[a]));             // the next tile's scores may come
+          constexpr uint32_t HIDDEN = 0xff800000u;         // -inf
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              if (!(lo >> e & 1u)) f[e] = -INFINITY;
-              if (!(hi >> e & 1u)) f[32 + e] = -INFINITY;
+          for (int h = 0; h < 2; ++h) {
+            const unsigned long long seen = h == 1 && !full ? 0ull : seen_from(key0 + 64 * h);
+            if (__any_sync(0xffffffffu, seen != ~0ull)) {
+              const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                if (!(lo >> e & 1u)) f[64 * h + e] = HIDDEN;
+                if (!(hi >> e & 1u)) f[64 * h + 32 + e] = HIDDEN;
+              }
             }
           }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], f[e]);
+          for (int e = 0; e < KEYS; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(f[e]));
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;        // sc > 0
-          grow = top > m_ref + 8.f || m_ref == -INFINITY;
+          const bool grow = top > m_ref + 8.f;
+          float alpha = 1.f;
           if (grow) {
-            const float base = fmaxf(m_ref, top);
-            alpha = base == -INFINITY ? 0.f : ex2(m_ref - base);
-            m_ref = base;
+            alpha = ex2(m_ref - top);
+            m_ref = top;
             l *= alpha;
           }
           const float neg = m_ref == -INFINITY ? 0.f : -m_ref;          // a row may see nothing of the tiles so far
           float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            f[e] = ex2(fmaf(f[e], sc, neg));
-            l4[e & 3] += f[e];
+          for (int e = 0; e < KEYS / 2; ++e) {
+            const float x = ex2(fmaf(__uint_as_float(f[2 * e]), sc, neg)), y = ex2(fmaf(__uint_as_float(f[2 * e + 1]), sc, neg));
+            l4[2 * e & 3] += x;
+            l4[(2 * e + 1) & 3] += y;
+            const __nv_bfloat162 t = __floats2bfloat162_rn(x, y);
+            f[e] = *reinterpret_cast<const uint32_t *>(&t);
           }
           l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+          // the product before has retired: its probabilities may be overwritten, and O is at rest
+          if (j > 0) {
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_full[a]), n_o & 1u, abort_flag, status, 0x6d))) { alive = false; break; }
+            ++n_o;
+            if (__any_sync(0xffffffffu, grow && mine)) {
+              tcgen05_fence_after();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const __nv_bfloat162 t = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
-            w[e] = *reinterpret_cast<const uint32_t *>(&t);
-          }
-        }
-        // the product before has retired: its probabilities may be overwritten, and O is at rest
-        if (j > 0 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_full[a]), (uint32_t)n_o & 1u, abort_flag, status, 0x6c))) { alive = false; break; }
-        n_o += j > 0;
-        if (busy) {
-          if (j > 0 && __any_sync(0xffffffffu, grow && mine)) {
-            tcgen05_fence_after();
+              for (int c = 0; c < DV; c += 32) {
+                uint32_t o[32];
+                tmem_ld_32x32b_x32(o_base + c, o);
+                tmem_ld_wait();
 #pragma unroll
-            for (int c = 0; c < DV; c += 32) {
-              uint32_t o[32];
-              tmem_ld_32x32b_x32(o_base + c, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st_32x32b_x32(o_base + c, o);
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                tmem_st_32x32b_x32(o_base + c, o);
+              }
+              tmem_st_wait();
             }
-            tmem_st_wait();
+          } else {
+            if (leader) store_read_wait();                 // nor does a store read them, of the item before
+            group_sync(1 + a);
           }
 #pragma unroll
-          for (int ch = 0; ch < 8; ++ch)
-            *reinterpret_cast<uint4 *>(prow + ((ch ^ (row & 7)) << 4)) = make_uint4(w[4 * ch], w[4 * ch + 1], w[4 * ch + 2], w[4 * ch + 3]);
+          for (int ch = 0; ch < KEYS / 8; ++ch) {
+            if (ch >= 8 && !full) break;
+            *reinterpret_cast<uint4 *>(prow + ch / 8 * BLOCK + ((ch % 8 ^ (row & 7)) << 4)) = make_uint4(f[4 * ch], f[4 * ch + 1], f[4 * ch + 2], f[4 * ch + 3]);
+          }
+        } else {                                           // no rows: only the barriers' counts
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&s_free[a]));
+          if (j > 0) {
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_full[a]), n_o & 1u, abort_flag, status, 0x6d))) { alive = false; break; }
+            ++n_o;
+          } else {
+            if (leader) store_read_wait();
+            group_sync(1 + a);
+          }
         }
         // keys of the tile that no row of the item sees: their values may be anything
-        if (a == 0 && !(key0 + KEYS <= it.span.first || (key0 >= it.span.from && key0 + KEYS <= it.span.end))) {
-          const int s = (g0 + j) % ST;
-          if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_full[s]), (uint32_t)((g0 + j) / ST) & 1u, abort_flag, status, 0x6d))) { alive = false; break; }
+        const int n_keys = full ? KEYS : 64;
+        if (a == 0 && !(key0 + n_keys <= it.span.first || (key0 >= it.span.from && key0 + n_keys <= it.span.end))) {
+          const int g = g0 + (j + 1 < it.tiles ? 2 * j + 2 : 2 * j + 1), s = g % ST;     // stage of V(j)
+          if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&kv_full[s]), (uint32_t)(g / ST) & 1u, abort_flag, status, 0x6e))) { alive = false; break; }
           for (int x = row; x < KEYS * (DV / 8); x += 128) {
             const int key = key0 + x % KEYS;
-            if (key >= it.span.first && (key < it.span.from || key >= it.span.end))
-              *reinterpret_cast<uint4 *>(v_s + s * Sh::V_BYTES + (x / KEYS / 8) * KV_BLOCK + (x % KEYS) * 128 + (x / KEYS % 8) * 16) = make_uint4(0, 0, 0, 0);
+            if (x % KEYS < n_keys && key >= it.span.first && (key < it.span.from || key >= it.span.end))
+              *reinterpret_cast<uint4 *>(kv_s + s * Sh::STAGE + (x / KEYS / 8) * BLOCK + (x % KEYS) * 128 + (x / KEYS % 8) * 16) = make_uint4(0, 0, 0, 0);
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");    // visible to the tensor core's reads
@@ -411,40 +475,46 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&p_full[a]));
       }
-      g0 += it.tiles;
+      g0 += 2 * it.tiles;
       if (!alive) break;
       if (it.tiles > 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_full[a]), (uint32_t)n_o & 1u, abort_flag, status, 0x6e))) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_full[a]), n_o & 1u, abort_flag, status, 0x6f))) break;
         ++n_o;
         tcgen05_fence_after();
       }
-      if (!busy) continue;
-      const int out_row = r0 + row;
-      const bool write = mine && !bad;
       if (p.m.splits == 1) {
-        const float f = l > 0.f ? p.m.out_scale / l : 0.f;
-        __nv_bfloat16 *dst = (__nv_bfloat16 *)p.m.out + (((size_t)it.s * p.m.mask.t + i) * p.m.heads + it.kvh * p.m.share + out_row % p.m.share) * DV;
+        // every item has tiles then; the probabilities' buffer takes the result, a block of 64 columns after the other
+        const float scale = l > 0.f ? p.m.out_scale / l : 0.f;
+        if (busy) {
 #pragma unroll
-        for (int c = 0; c < DV; c += 32) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(o_base + c, o);
-          tmem_ld_wait();
-          if (write) {
+          for (int c = 0; c < DV; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(o_base + c, o);
+            tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
-              uint32_t v[4];
+              uint32_t w[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                const __nv_bfloat162 t = __floats2bfloat162_rn(__uint_as_float(o[e + 2 * k]) * f, __uint_as_float(o[e + 2 * k + 1]) * f);
-                v[k] = *reinterpret_cast<const uint32_t *>(&t);
+                const __nv_bfloat162 t = __floats2bfloat162_rn(__uint_as_float(o[e + 2 * k]) * scale, __uint_as_float(o[e + 2 * k + 1]) * scale);
+                w[k] = *reinterpret_cast<const uint32_t *>(&t);
               }
-              *reinterpret_cast<uint4 *>(dst + c + e) = make_uint4(v[0], v[1], v[2], v[3]);
+              *reinterpret_cast<uint4 *>(prow + c / CB * BLOCK + (((c + e) % CB / 8 ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
         }
-      } else {
-        const size_t slot = ((size_t)it.slice * p.pairs + it.s * p.m.kv_heads + it.kvh) * p.m.rows + out_row;
-        if (write) p.m.part_ml[slot] = make_float2(m_ref, l);
+        tcgen05_fence_before();                            // the loads of O are done before this group's next p_full lets it be overwritten
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        group_sync(1 + a);
+        if (leader && !bad) {
+          for (int c = 0; c < DV / CB; ++c) tma_store_4d(&tmO, smem_u32(p_group + c * BLOCK), c * CB, it.kvh * p.m.share, r0 / p.m.share, it.s);
+          store_commit();
+        }
+      } else if (busy) {
+        const size_t pair = (size_t)it.slice * p.pairs + it.s * p.m.kv_heads + it.kvh;
+        const int out_row = r0 + row;
+        const bool write = mine && !bad;
+        if (write) p.m.part_ml[pair * p.m.rows + out_row] = make_float2(m_ref, l);
         if (it.tiles > 0) {
 #pragma unroll
           for (int c = 0; c < DV; c += 32) {
@@ -453,13 +523,15 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
             tmem_ld_wait();
             if (write) {
 #pragma unroll
-              for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4 *>(p.m.part_o + slot * DV + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<uint4 *>(p.m.part_o + (pair * (DV / 4) + (c + e) / 4) * p.m.rows + out_row) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
           }
         }
+        tcgen05_fence_before();
       }
-      tcgen05_fence_before();                              // the loads of O are done before this group's next p_full lets it be overwritten
     }
+    if (leader) store_wait();                              // before the shared memory goes
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -477,22 +549,22 @@ int32_t launch(ugb_device *dev, const ugb_masked_attention_args &a, const Params
     UGB_CUDA(dev, cudaFuncSetAttribute(masked_attention_tc_kernel<DQ, DV, RT, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM_BYTES));
     attr_set[dev->ordinal & 63] = true;
   }
-  CUtensorMap tmQ, tmK, tmV;
+  CUtensorMap tmQ, tmK, tmV, tmO;
   int32_t rc;
-  {   // q [b, t, heads, DQ]: a box is 64 columns of the heads of a group for as many positions as 128 rows hold
-    const uint64_t dims[4] = {(uint64_t)DQ, (uint64_t)a.heads, (uint64_t)a.t, (uint64_t)a.b};
-    const uint64_t strides[3] = {(uint64_t)DQ, (uint64_t)a.heads * DQ, (uint64_t)a.t * a.heads * DQ};
+  auto q_map = [&](CUtensorMap *m, const void *base, int d) {      // [b, t, heads, d]: a box is 64 columns of a group's heads for as many positions as 128 rows hold
+    const uint64_t dims[4] = {(uint64_t)d, (uint64_t)a.heads, (uint64_t)a.t, (uint64_t)a.b};
+    const uint64_t strides[3] = {(uint64_t)d, (uint64_t)a.heads * d, (uint64_t)a.t * a.heads * d};
     const uint32_t box[4] = {(uint32_t)CB, (uint32_t)p.m.share, (uint32_t)(p.per_group / p.m.share), 1};
-    if ((rc = ugb_tc_encode_bf16(dev, &tmQ, (const __nv_bfloat16 *)a.q, 4, dims, strides, box))) return rc;
-  }
+    return ugb_tc_encode_bf16(dev, m, (const __nv_bfloat16 *)base, 4, dims, strides, box);
+  };
   auto kv_map = [&](CUtensorMap *m, const void *base, int d) {     // [b, kv_heads, t_max, d]
     const uint64_t dims[4] = {(uint64_t)d, (uint64_t)a.kv_heads, (uint64_t)a.t_max, (uint64_t)a.b};
     const uint64_t strides[3] = {(uint64_t)a.t_max * d, (uint64_t)d, (uint64_t)a.kv_heads * a.t_max * d};
-    const uint32_t box[4] = {(uint32_t)CB, 1, (uint32_t)KEYS, 1};
+    const uint32_t box[4] = {(uint32_t)CB, 1, 64, 1};
     return ugb_tc_encode_bf16(dev, m, (const __nv_bfloat16 *)base, 4, dims, strides, box);
   };
-  if ((rc = kv_map(&tmK, a.k, DQ)) || (rc = kv_map(&tmV, a.v, DV))) return rc;
-  masked_attention_tc_kernel<DQ, DV, RT, TREE><<<(unsigned)((long long)p.row_tiles * p.pairs * p.m.splits), Sh::THREADS, Sh::SMEM_BYTES, dev->stream>>>(tmQ, tmK, tmV, p);
+  if ((rc = q_map(&tmQ, a.q, DQ)) || (rc = q_map(&tmO, a.out, DV)) || (rc = kv_map(&tmK, a.k, DQ)) || (rc = kv_map(&tmV, a.v, DV))) return rc;
+  masked_attention_tc_kernel<DQ, DV, RT, TREE><<<(unsigned)((long long)p.row_tiles * p.pairs * p.m.splits), Sh::THREADS, Sh::SMEM_BYTES, dev->stream>>>(tmQ, tmK, tmV, tmO, p);
   return ugb_after_launch(dev, "masked_attention_tc_kernel");
 }
 
