@@ -67,7 +67,10 @@ masked_attention_generic_kernel(Params p) {
   float *qs = gsm, *ks = qs + TR * kld, *vs = ks + KEYS * kld, *ps = vs + KEYS * vld;
   const int s = blockIdx.y / p.kv_heads, kvh = blockIdx.y % p.kv_heads, row0 = blockIdx.x * TR, n_rows = min(TR, p.rows - row0);
   const int pos = p.mask.pos[s];
-  if (!check_sequence<TREE>(p.mask, s, pos, up, p.status)) return;
+  if (!check_sequence<TREE>(p.mask, s, pos, up, p.status)) {
+    if (p.splits > 1 && blockIdx.z == 0 && (int)threadIdx.x < n_rows) p.part_ml[(size_t)blockIdx.y * p.rows + row0 + threadIdx.x] = make_float2(NAN, 0.f);
+    return;
+  }
   if constexpr (TREE) {
     for (int r = threadIdx.x; r < TR; r += 256) {
       uint32_t w[4] = {0, 0, 0, 0};
@@ -218,47 +221,45 @@ masked_attention_generic_kernel(Params p) {
 }
 
 // ------------------------------------------------------------- combine ------
-// One CTA per 32 rows of a pair: lane = row, warp = columns.  The slices in their order, whatever order they ran in.
-template <typename T, bool TREE>
+// One CTA per 32 rows of a pair and 32 columns: lane = row, warp = 4 columns.  The slices in their order, whatever order they ran in.  A maximum that is
+// NaN marks a row that was not computed and is left as it is.
+template <typename T>
 __global__ void __launch_bounds__(256)
 masked_combine_kernel(Params p, int pairs) {
-  __shared__ float weight[UGB_MASKED_SPLITS][32], whole[32];
-  __shared__ T done[32][256 + 8];
-  __shared__ int up[TREE ? UGB_TREE_MAX : 1];
+  __shared__ T done[32][32 + 8];
   const int blocks = (p.rows + 31) / 32, pair = blockIdx.x / blocks, row0 = blockIdx.x % blocks * 32, n_rows = min(32, p.rows - row0);
   const int s = pair / p.kv_heads, kvh = pair % p.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = row0 + min(lane, n_rows - 1);
-  if (!check_sequence<TREE>(p.mask, s, p.mask.pos[s], up, p.status)) return;     // nothing was computed
-  const size_t n = (size_t)pairs * p.rows, at = (size_t)pair * p.rows + row;
-  if (warp == 0) {
-    float m = -INFINITY, l = 0.f;
-    for (int z = 0; z < p.splits; ++z) m = fmaxf(m, p.part_ml[z * n + at].x);
-    for (int z = 0; z < p.splits; ++z) {
-      const float2 ml = p.part_ml[z * n + at];
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-      weight[z][lane] = f;
-      l = fmaf(f, ml.y, l);
-    }
-    whole[lane] = l > 0.f ? p.out_scale / l : 0.f;
+  const int c = min(blockIdx.y * 8 + warp, p.dv / 4 - 1);  // four columns; the last warps repeat one where dv ends
+  const size_t n = (size_t)pairs * p.rows, step = (size_t)pairs * (p.dv / 4) * p.rows;
+  const float2 *ml = p.part_ml + (size_t)pair * p.rows + row;
+  const float4 *o = p.part_o + ((size_t)pair * (p.dv / 4) + c) * p.rows + row;
+  float m = -INFINITY, l = 0.f;
+  bool left = false;
+#pragma unroll 8
+  for (int z = 0; z < p.splits; ++z) {
+    const float x = ml[z * n].x;
+    left |= x != x;
+    m = fmaxf(m, x);
   }
-  __syncthreads();
-  const float f = whole[lane];
-  for (int c = warp; c < p.dv / 4; c += 8) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int z = 0; z < p.splits; ++z) {
-      const float w = weight[z][lane];
-      if (w > 0.f) {                                       // what weighs nothing was not written either
-        const float4 v = p.part_o[(((size_t)z * pairs + pair) * (p.dv / 4) + c) * p.rows + row];
-        acc.x = fmaf(w, v.x, acc.x); acc.y = fmaf(w, v.y, acc.y); acc.z = fmaf(w, v.z, acc.z); acc.w = fmaf(w, v.w, acc.w);
-      }
-    }
-    done[lane][4 * c] = (T)(acc.x * f); done[lane][4 * c + 1] = (T)(acc.y * f); done[lane][4 * c + 2] = (T)(acc.z * f); done[lane][4 * c + 3] = (T)(acc.w * f);
+  if (__all_sync(0xffffffffu, left)) return;               // rows of one sequence: all of them or none, in every warp
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int z = 0; z < p.splits; ++z) {
+    const float2 w = ml[z * n];
+    const bool some = w.x != -INFINITY;                    // otherwise nothing was seen, or written
+    const float4 v = some ? o[z * step] : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float f = some ? ex2(w.x - m) : 0.f;
+    l = fmaf(f, w.y, l);
+    acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
   }
+  const float f = l > 0.f ? p.out_scale / l : 0.f;
+  T *d = &done[lane][4 * warp];
+  d[0] = (T)(acc.x * f); d[1] = (T)(acc.y * f); d[2] = (T)(acc.z * f); d[3] = (T)(acc.w * f);
   __syncthreads();
+  const int column = blockIdx.y * 32 + lane;
   for (int r = warp; r < n_rows; r += 8) {
     const int i = (row0 + r) / p.share, h = (row0 + r) % p.share;
-    T *out = (T *)p.out + (((size_t)s * p.mask.t + i) * p.heads + kvh * p.share + h) * p.dv;
-    for (int c = lane; c < p.dv; c += 32) out[c] = done[r][c];
+    if (column < p.dv) ((T *)p.out)[(((size_t)s * p.mask.t + i) * p.heads + kvh * p.share + h) * p.dv + column] = done[r][lane];
   }
 }
 
@@ -287,9 +288,19 @@ template <typename T, bool COPIES> cudaError_t launch_rows(bool tree, int rm, di
   return tree ? launch_columns<T, 4, true, COPIES>(grid, smem, st, p) : launch_columns<T, 4, false, COPIES>(grid, smem, st, p);
 }
 
-// Slices of the keys: as many as bring the CTAs to `slots`, of at least two tiles each (a slice costs a round of sums through memory).
-int slices(long long ctas, long long slots, int tiles) {
-  return (int)std::max(1LL, std::min({slots / std::max(1LL, ctas), (long long)(tiles + 1) / 2, (long long)UGB_MASKED_SPLITS}));
+// Slices of the keys, for `items` CTAs' worth of work of `tiles` tiles of 64 keys each on `slots`: what is shortest, in tiles, for the CTA that has most to do,
+// where an item's start takes `start` tiles, twice that when its sums leave through memory, and joining them half a tile per slice (measured: 24 nodes
+// over 2000 positions in 4 / 6 / 8 / 12 slices 22.5 / 20.5 / 18.5 / 20.5 us, 64 nodes of 16 sequences over 8192 in 1 / 2 / 4 168 / 193 / 198 us, f32 in
+// 1 / 2 / 3 / 4, a block of 777, 135 / 121 / 118 / 125 us).
+int slices(long long items, long long slots, int tiles, int parts, int start) {
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s * parts <= UGB_MASKED_SPLITS && (s == 1 || tiles >= 2 * s); ++s) {
+    const long long rounds = (items * s + slots - 1) / slots;
+    const double all = (double)rounds * ((tiles + s - 1) / s + (s > 1 ? 2 * start : start)) + (s > 1 ? 0.25 * s * (1 + parts) : 0.0);
+    if (all < least) { least = all; best = s; }
+  }
+  return best;
 }
 
 }  // namespace
@@ -302,20 +313,22 @@ int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a
   p.mask = ugb_mask{a.pos, a.parents, a.t, a.t_max, a.sinks, a.window};
   p.heads = a.heads; p.kv_heads = a.kv_heads; p.share = a.heads / a.kv_heads; p.rows = a.t * p.share; p.dq = a.dq; p.dv = a.dv;
   p.scale = a.scale * LOG2E; p.out_scale = a.out_scale; p.part_o = nullptr; p.part_ml = nullptr; p.status = dev->status_dev;
-  // the most keys that a row of tiles can see: the position is on the device
-  const long long reach = tree ? a.t_max : std::min<long long>(a.t_max, (long long)a.window + a.t + a.sinks);
-  const int tiles = (int)((reach + KEYS - 1) / KEYS + 1), pairs = a.b * a.kv_heads;
+  const int pairs = a.b * a.kv_heads;
   const bool tc = ugb_masked_tc_takes(a);
   const int rm = p.rows <= 16 ? 1 : 4, row_tiles = (p.rows + 16 * rm - 1) / (16 * rm);
-  long long ctas = (long long)row_tiles * pairs, slots = 2LL * dev->sm_count;
-  if (tc) ugb_masked_tc_shape(dev, a, &ctas, &slots);
-  p.splits = slices(ctas, slots, tiles);
+  long long items = (long long)row_tiles * pairs, slots = 2LL * dev->sm_count;
+  int parts = 1, positions = 16 * rm / p.share + 1;
+  if (tc) ugb_masked_tc_shape(dev, a, &items, &slots, &parts, &positions);
+  // the most keys that the rows of an item can see: their positions are on the device
+  const long long reach = tree ? a.t_max : std::min<long long>(a.t_max, (long long)a.window + std::min(positions, a.t) + a.sinks);
+  p.splits = slices(items, slots, (int)((reach + 63) / 64), parts, tc ? 6 : 0);
+  const int sums = p.splits * parts;
   const size_t n = (size_t)pairs * p.rows;
   void *work = nullptr;
-  if (p.splits > 1) {
-    UGB_CUDA(dev, ugb_malloc_async(dev, &work, (size_t)p.splits * n * (size_t)(a.dv + 2) * 4));
+  if (sums > 1) {
+    UGB_CUDA(dev, ugb_malloc_async(dev, &work, (size_t)sums * n * (size_t)(a.dv + 2) * 4));
     p.part_o = (float4 *)work;
-    p.part_ml = (float2 *)((float *)work + (size_t)p.splits * n * a.dv);
+    p.part_ml = (float2 *)((float *)work + (size_t)sums * n * a.dv);
   }
   int32_t rc;
   if (tc) {
@@ -329,10 +342,11 @@ int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a
     rc = e != cudaSuccess ? ugb_fail(dev, UGB_ERR_CUDA, "launch of masked_attention_generic_kernel failed: %s", cudaGetErrorString(e))
                           : ugb_after_launch(dev, "masked_attention_generic_kernel");
   }
-  if (rc == UGB_OK && p.splits > 1) {
-    const dim3 rows((unsigned)(pairs * ((p.rows + 31) / 32)));
-    if (a.f32) tree ? masked_combine_kernel<float, true><<<rows, 256, 0, dev->stream>>>(p, pairs) : masked_combine_kernel<float, false><<<rows, 256, 0, dev->stream>>>(p, pairs);
-    else tree ? masked_combine_kernel<__nv_bfloat16, true><<<rows, 256, 0, dev->stream>>>(p, pairs) : masked_combine_kernel<__nv_bfloat16, false><<<rows, 256, 0, dev->stream>>>(p, pairs);
+  if (rc == UGB_OK && sums > 1) {
+    p.splits = sums;
+    const dim3 rows((unsigned)(pairs * ((p.rows + 31) / 32)), (unsigned)((a.dv + 31) / 32));
+    if (a.f32) masked_combine_kernel<float><<<rows, 256, 0, dev->stream>>>(p, pairs);
+    else masked_combine_kernel<__nv_bfloat16><<<rows, 256, 0, dev->stream>>>(p, pairs);
     rc = ugb_after_launch(dev, "masked_combine_kernel");
   }
   if (work) cudaFreeAsync(work, dev->stream);

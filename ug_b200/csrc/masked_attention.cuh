@@ -21,7 +21,7 @@ struct ugb_mask {
   const int *pos, *parents;
   int t, t_max, sinks, window;
 };
-constexpr int UGB_MASKED_SPLITS = 64;    // slices of the keys, at most
+constexpr int UGB_MASKED_SPLITS = 256;    // slices of the keys and their parts, at most
 struct ugb_masked_params {
   const void *q, *k, *v;
   void *out;
@@ -58,9 +58,10 @@ template <bool TREE> __device__ __forceinline__ Span span_of(const ugb_mask &m, 
 }  // namespace ugb_masked
 #endif
 
-// The tensor-core kernel (masked_attention_tc.cu).  Whether it takes a call; how many CTAs it makes of it and how many run at a time; its launch.
+// The tensor-core kernel (masked_attention_tc.cu).  Whether it takes a call; how many items a slice of the keys has, how many run at a time, into
+// how many parts each leaves its slice's result and how many query positions it has; its launch.
 bool ugb_masked_tc_takes(const ugb_masked_attention_args &a);
-void ugb_masked_tc_shape(const ugb_device *dev, const ugb_masked_attention_args &a, long long *ctas, long long *slots);
+void ugb_masked_tc_shape(const ugb_device *dev, const ugb_masked_attention_args &a, long long *items, long long *slots, int *parts, int *positions);
 int32_t ugb_masked_tc_launch(ugb_device *dev, const ugb_masked_attention_args &a, const ugb_masked_params &p);
 
 int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a);

@@ -8,6 +8,8 @@
 // The scores of the next tile are formed as soon as this tile's are in registers, so that the softmax finds them ready; while one group's softmax runs, the
 // other's products do.  O stays in TMEM from the first tile to the last: it is rescaled only where a row's maximum has grown by more than 2^8 since
 // it was last (the probabilities are then up to 2^8, which costs bf16 no precision, and the sum is f32), which after the first tiles is hardly ever.
+// Up to 32 rows (single positions, small trees) lie four times in the tile, once for each softmax warp, which takes a quarter of every tile's keys: a
+// warp's chain per tile is then short enough for HBM.  The quarters are joined as slices of the keys are, by the combine kernel.
 // Results leave through shared memory, by TMA.  Rows of V that no row of the item sees are set to zero there: P is zero for them, but 0 x NaN is not.
 // Grid: one CTA per item; a CTA that is done takes over the item of one that has not started (cluster launch control), so that its set-up and its
 // TMEM are shared by many and long and short items even out.  Every wait on an mbarrier is bounded.
@@ -32,20 +34,21 @@ constexpr int KEYS = 128;                                  // of a tile
 constexpr int BLOCK = 128 * CB * 2;                        // 128 rows of 64 columns: 16 KiB
 constexpr int P_BYTES = 2 * BLOCK;                         // 128 rows x 128 keys
 
-template <int DQ, int DV, int RT> struct Shape {
+// RT 0: up to 32 rows, spread over the four warps of one group.
+template <int DQ, int DV, int RT0> struct Shape {
+  static constexpr int RT = RT0 ? RT0 : 1;
   static constexpr int THREADS = 64 + 128 * RT;
   static constexpr int Q_BYTES = DQ / CB * BLOCK, STAGE = (DQ > DV ? DQ : DV) / CB * BLOCK;     // a stage holds a tile of keys or of values
   static constexpr int O_COL = RT * KEYS;                  // TMEM: S [RT][128], then O [RT][DV]
   static constexpr int TMEM_USED = O_COL + RT * DV, TMEM_COLS = TMEM_USED <= 256 ? 256 : 512;
-  static constexpr int FIXED = RT * (Q_BYTES + P_BYTES) + 1024 /*alignment*/ + 512 /*barriers*/;
-  // one group of 64-wide heads: two CTAs per SM, since one softmax warp per tile does not keep up with HBM
-  static constexpr int CTAS_PER_SM = RT == 1 && DQ + DV == 128 ? 2 : 1;
-  static constexpr int LIMIT = CTAS_PER_SM == 2 ? 112 * 1024 : 225 * 1024 + 512;
+  static constexpr int FIXED = RT * (Q_BYTES + P_BYTES) + 512 /*barriers*/ + RT * UGB_TREE_MAX * 4;
+  static constexpr int CTAS_PER_SM = RT0 <= 1 && DQ + DV == 128 ? 2 : 1;      // more would not fit
+  static constexpr int LIMIT = (CTAS_PER_SM == 2 ? 113 : 227) * 1024;
   static constexpr int FIT = (LIMIT - FIXED) / STAGE, STAGES = FIT > 8 ? 8 : FIT;
   static constexpr int TILES = FIXED + STAGES * STAGE;
   // a CTA that takes all of the TMEM is alone on its SM: more than half of the shared memory sees to that
   static constexpr int SMEM_BYTES = CTAS_PER_SM == 1 && TILES < 116 * 1024 ? 116 * 1024 : TILES;
-  static_assert(TMEM_USED <= 512 && STAGES >= 3 && SMEM_BYTES <= 226 * 1024, "tile shape");
+  static_assert(TMEM_USED <= 512 && STAGES >= 3 && SMEM_BYTES <= 227 * 1024, "tile shape");
 };
 
 struct Params {
@@ -138,15 +141,18 @@ template <int RT, bool TREE> __device__ __forceinline__ Item item_of(int idx, co
   return it;
 }
 
-template <int DQ, int DV, int RT, bool TREE>
-__global__ void __launch_bounds__((Shape<DQ, DV, RT>::THREADS), (Shape<DQ, DV, RT>::CTAS_PER_SM))
+template <int DQ, int DV, int RT0, bool TREE>
+__global__ void __launch_bounds__((Shape<DQ, DV, RT0>::THREADS), (Shape<DQ, DV, RT0>::CTAS_PER_SM))
 masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                            const __grid_constant__ CUtensorMap tmO, Params p) {
-  using Sh = Shape<DQ, DV, RT>;
-  constexpr int ST = Sh::STAGES;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ int up[TREE ? RT : 1][TREE ? UGB_TREE_MAX : 1];
-  uint8_t *smem = (uint8_t *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  using Sh = Shape<DQ, DV, RT0>;
+  constexpr int ST = Sh::STAGES, RT = Sh::RT;
+  constexpr bool SPREAD = RT0 == 0;
+  extern __shared__ __align__(1024) uint8_t smem[];        // all of it: a block of rows starts at a multiple of 1024 bytes
+  if (smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0 && atomicCAS(&p.m.status->code, 0u, (unsigned)UGB_ERR_UNSUPPORTED) == 0u) p.m.status->detail = 0x5f;
+    return;
+  }
   uint8_t *q_s = smem, *p_s = q_s + RT * Sh::Q_BYTES, *kv_s = p_s + RT * P_BYTES;
   uint64_t *bars = (uint64_t *)(kv_s + ST * Sh::STAGE);
   uint64_t *q_full = bars, *q_empty = bars + 1, *answer_full = bars + 2, *answer = bars + 4;       // the answer: 16 bytes, aligned
@@ -154,6 +160,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
   uint64_t *kv_full = o_full + RT, *kv_empty = kv_full + ST;
   uint32_t *tmem_slot = (uint32_t *)(kv_empty + ST);
   volatile int *abort_flag = (volatile int *)(tmem_slot + 1), *item_slot = (volatile int *)(tmem_slot + 2);      // two entries
+  int(*up)[UGB_TREE_MAX] = (int(*)[UGB_TREE_MAX])((uint8_t *)bars + 512);
   static_assert((10 + 4 * RT + 2 * ST) * 8 + 16 <= 512, "barriers fit");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -182,6 +189,10 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmK) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmV) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmO) : "memory");
+  }
+  if constexpr (SPREAD) {                                  // a row's probabilities outside its warp's quarter of the keys stay zero
+    for (int i = threadIdx.x; i < P_BYTES / 16; i += Sh::THREADS) reinterpret_cast<uint4 *>(p_s)[i] = make_uint4(0, 0, 0, 0);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(Sh::TMEM_COLS) : "memory");
@@ -223,10 +234,12 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
           alive = mbar_wait(smem_u32(q_empty), ((uint32_t)n_q & 1u) ^ 1u, abort_flag, status, 0x62);
           ++n_q;
           if (alive) {
-            mbar_expect_tx(smem_u32(q_full), (uint32_t)(RT * (DQ / CB) * p.per_group * CB * 2));
-            for (int a = 0; a < RT; ++a)
+            constexpr int COPIES = SPREAD ? 4 : RT;        // rows 32 apart, or groups
+            mbar_expect_tx(smem_u32(q_full), (uint32_t)(COPIES * (DQ / CB) * p.per_group * CB * 2));
+            for (int a = 0; a < COPIES; ++a)
               for (int c = 0; c < DQ / CB; ++c)
-                tma_load_4d(smem_u32(q_s + a * Sh::Q_BYTES + c * BLOCK), &tmQ, smem_u32(q_full), c * CB, it.kvh * p.m.share, i0 + a * step, it.s);
+                tma_load_4d(smem_u32(q_s + a * (SPREAD ? 32 * 128 : Sh::Q_BYTES) + c * BLOCK), &tmQ, smem_u32(q_full), c * CB, it.kvh * p.m.share,
+                            SPREAD ? i0 : i0 + a * step, it.s);
             load(&tmK, DQ, 0);
           }
           for (int j = 0; j < it.tiles && alive; ++j) {
@@ -321,11 +334,13 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16), s_base = lane_base + (uint32_t)(a * KEYS), o_base = lane_base + (uint32_t)(Sh::O_COL + a * DV);
     uint8_t *const p_group = p_s + a * P_BYTES, *const prow = p_group + row * 128;
     const bool leader = threadIdx.x == 64 + a * 128;       // issues the group's stores
+    bool alive = true;
     int g0 = 0;                                            // stages of the CTA so far
     uint32_t n_s = 0, n_o = 0;                             // S and O products of this group so far
     for (int n_it = 0;; ++n_it) {
       const int at = n_it & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&item_full[at]), (uint32_t)(n_it >> 1) & 1u, abort_flag, status, 0x6b))) break;
+      alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&item_full[at]), (uint32_t)(n_it >> 1) & 1u, abort_flag, status, 0x6b));
+      if (!alive) break;
       const int idx = item_slot[at];
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&item_empty[at]));
@@ -333,13 +348,17 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
       const Item it = item_of<RT, TREE>(idx, p);
       if (!it.valid) {
         if (it.pos != -1 && threadIdx.x == 64) raise_invalid(status, it.s);
+        const int r = it.row0 + a * p.per_group + (SPREAD ? lane : row);
+        if (p.m.part_ml && it.slice == 0 && r < p.m.rows && (!SPREAD || quad == 0) && (SPREAD || row < p.per_group))
+          p.m.part_ml[((size_t)it.s * p.m.kv_heads + it.kvh) * p.m.rows + r] = make_float2(NAN, 0.f);       // for the combine kernel: to be left as it is
         continue;
       }
       const int r0 = it.row0 + a * p.per_group, n_rows = min(p.per_group, p.m.rows - r0);      // of this group
       if (n_rows <= 0) { g0 += 2 * it.tiles; continue; }
-      const bool mine = row < n_rows;                      // this thread has a row
-      const bool busy = quad * 32 < n_rows;                // this warp has rows
-      const int i = (r0 + min(row, n_rows - 1)) / p.m.share, n = it.pos + i;
+      const int in_rows = SPREAD ? lane : row;
+      const bool mine = in_rows < n_rows;                  // this thread has a row
+      const bool busy = SPREAD || quad * 32 < n_rows;      // this warp has rows
+      const int i = (r0 + min(in_rows, n_rows - 1)) / p.m.share, n = it.pos + i;
       unsigned long long nodes0 = 0, nodes1 = 0;
       bool bad = false;
       if constexpr (TREE) {
@@ -369,13 +388,78 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
       };
       const float sc = p.m.scale;
       float m_ref = -INFINITY, l = 0.f;
-      bool alive = true;
       for (int j = 0; j < it.tiles; ++j) {
         const int key0 = it.key0(j);
         const bool full = it.full(j);
         if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[a]), n_s & 1u, abort_flag, status, 0x6c))) { alive = false; break; }
         ++n_s;
-        if (busy) {
+        if constexpr (SPREAD) {
+          const bool some = full || quad < 2;              // a half tile has keys for two warps
+          if (some) {
+            tcgen05_fence_after();
+            uint32_t f[32];
+            tmem_ld_32x32b_x32(s_base + 32 * quad, f);
+            tmem_ld_wait();
+            tcgen05_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&s_free[a]));
+            const uint32_t on = (uint32_t)(seen_from(key0 + 64 * (quad / 2)) >> (32 * (quad & 1)));
+            if (__any_sync(0xffffffffu, on != ~0u)) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!(on >> e & 1u)) f[e] = 0xff800000u;   // -inf
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(f[e]));
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+            const bool grow = top > m_ref + 8.f;
+            float alpha = 1.f;
+            if (grow) {
+              alpha = ex2(m_ref - top);
+              m_ref = top;
+              l *= alpha;
+            }
+            const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
+            float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float x = ex2(fmaf(__uint_as_float(f[2 * e]), sc, neg)), y = ex2(fmaf(__uint_as_float(f[2 * e + 1]), sc, neg));
+              l4[2 * e & 3] += x;
+              l4[(2 * e + 1) & 3] += y;
+              const __nv_bfloat162 t = __floats2bfloat162_rn(x, y);
+              f[e] = *reinterpret_cast<const uint32_t *>(&t);
+            }
+            l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+            if (j > 0) {
+              if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_full[a]), n_o & 1u, abort_flag, status, 0x6d))) { alive = false; break; }
+              ++n_o;
+              if (__any_sync(0xffffffffu, grow && mine)) {
+                tcgen05_fence_after();
+#pragma unroll
+                for (int c = 0; c < DV; c += 32) {
+                  uint32_t o[32];
+                  tmem_ld_32x32b_x32(o_base + c, o);
+                  tmem_ld_wait();
+#pragma unroll
+                  for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                  tmem_st_32x32b_x32(o_base + c, o);
+                }
+                tmem_st_wait();
+              }
+            }
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch)
+              *reinterpret_cast<uint4 *>(prow + quad / 2 * BLOCK + (((quad % 2 * 4 + ch) ^ (row & 7)) << 4)) = make_uint4(f[4 * ch], f[4 * ch + 1], f[4 * ch + 2], f[4 * ch + 3]);
+          } else {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&s_free[a]));
+            if (j > 0) {
+              if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_full[a]), n_o & 1u, abort_flag, status, 0x6d))) { alive = false; break; }
+              ++n_o;
+            }
+          }
+        } else if (busy) {
           tcgen05_fence_after();
           uint32_t f[KEYS];                                // scores, and in their place, two to a register, the probabilities
           {
@@ -478,11 +562,12 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
       g0 += 2 * it.tiles;
       if (!alive) break;
       if (it.tiles > 0) {
-        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_full[a]), n_o & 1u, abort_flag, status, 0x6f))) break;
+        alive = __all_sync(0xffffffffu, mbar_wait(smem_u32(&o_full[a]), n_o & 1u, abort_flag, status, 0x6f));
+        if (!alive) break;
         ++n_o;
         tcgen05_fence_after();
       }
-      if (p.m.splits == 1) {
+      if (!SPREAD && p.m.splits == 1) {
         // every item has tiles then; the probabilities' buffer takes the result, a block of 64 columns after the other
         const float scale = l > 0.f ? p.m.out_scale / l : 0.f;
         if (busy) {
@@ -511,10 +596,10 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
           store_commit();
         }
       } else if (busy) {
-        const size_t pair = (size_t)it.slice * p.pairs + it.s * p.m.kv_heads + it.kvh;
-        const int out_row = r0 + row;
+        const size_t pair = (size_t)(SPREAD ? 4 * it.slice + quad : it.slice) * p.pairs + it.s * p.m.kv_heads + it.kvh;
+        const int out_row = r0 + in_rows;
         const bool write = mine && !bad;
-        if (write) p.m.part_ml[pair * p.m.rows + out_row] = make_float2(m_ref, l);
+        if (mine) p.m.part_ml[pair * p.m.rows + out_row] = make_float2(bad ? NAN : m_ref, l);
         if (it.tiles > 0) {
 #pragma unroll
           for (int c = 0; c < DV; c += 32) {
@@ -532,6 +617,8 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
       }
     }
     if (leader) store_wait();                              // before the shared memory goes
+    // a wait gave up: the warps that are still at a barrier of the group's leave it, and give up too
+    if (!alive) asm volatile("barrier.cta.arrive %0, 128;" ::"r"(1 + a) : "memory");
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -541,12 +628,12 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
   }
 }
 
-template <int DQ, int DV, int RT, bool TREE>
+template <int DQ, int DV, int RT0, bool TREE>
 int32_t launch(ugb_device *dev, const ugb_masked_attention_args &a, const Params &p) {
-  using Sh = Shape<DQ, DV, RT>;
+  using Sh = Shape<DQ, DV, RT0>;
   static bool attr_set[64] = {};
   if (!attr_set[dev->ordinal & 63]) {
-    UGB_CUDA(dev, cudaFuncSetAttribute(masked_attention_tc_kernel<DQ, DV, RT, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM_BYTES));
+    UGB_CUDA(dev, cudaFuncSetAttribute(masked_attention_tc_kernel<DQ, DV, RT0, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::SMEM_BYTES));
     attr_set[dev->ordinal & 63] = true;
   }
   CUtensorMap tmQ, tmK, tmV, tmO;
@@ -564,21 +651,26 @@ int32_t launch(ugb_device *dev, const ugb_masked_attention_args &a, const Params
     return ugb_tc_encode_bf16(dev, m, (const __nv_bfloat16 *)base, 4, dims, strides, box);
   };
   if ((rc = q_map(&tmQ, a.q, DQ)) || (rc = q_map(&tmO, a.out, DV)) || (rc = kv_map(&tmK, a.k, DQ)) || (rc = kv_map(&tmV, a.v, DV))) return rc;
-  masked_attention_tc_kernel<DQ, DV, RT, TREE><<<(unsigned)((long long)p.row_tiles * p.pairs * p.m.splits), Sh::THREADS, Sh::SMEM_BYTES, dev->stream>>>(tmQ, tmK, tmV, tmO, p);
+  masked_attention_tc_kernel<DQ, DV, RT0, TREE><<<(unsigned)((long long)p.row_tiles * p.pairs * p.m.splits), Sh::THREADS, Sh::SMEM_BYTES, dev->stream>>>(tmQ, tmK, tmV, tmO, p);
   return ugb_after_launch(dev, "masked_attention_tc_kernel");
 }
 
-int groups_of(const ugb_masked_attention_args &a) { return a.t > 128 / (a.heads / a.kv_heads) ? 2 : 1; }
+// Groups of 128 rows in a CTA; 0: up to 32 rows in all.
+int groups_of(const ugb_masked_attention_args &a) {
+  const int share = a.heads / a.kv_heads;
+  return a.t * share <= 32 ? 0 : a.t > 128 / share ? 2 : 1;
+}
 int per_group(const ugb_masked_attention_args &a) {
   const int share = a.heads / a.kv_heads;
-  return share * (128 / share);
+  return groups_of(a) == 0 ? share * a.t : share * (128 / share);
 }
 int row_tiles(const ugb_masked_attention_args &a) {
-  const int per = per_group(a) * groups_of(a);
+  const int per = per_group(a) * std::max(1, groups_of(a));
   return (a.t * (a.heads / a.kv_heads) + per - 1) / per;
 }
 
 template <int DQ, int DV> int32_t launch_any(ugb_device *dev, const ugb_masked_attention_args &a, const Params &p) {
+  if (groups_of(a) == 0) return a.parents ? launch<DQ, DV, 0, true>(dev, a, p) : launch<DQ, DV, 0, false>(dev, a, p);
   if (groups_of(a) == 1) return a.parents ? launch<DQ, DV, 1, true>(dev, a, p) : launch<DQ, DV, 1, false>(dev, a, p);
   return a.parents ? launch<DQ, DV, 2, true>(dev, a, p) : launch<DQ, DV, 2, false>(dev, a, p);
 }
@@ -589,12 +681,14 @@ bool ugb_masked_tc_takes(const ugb_masked_attention_args &a) {
   const bool wide = (a.dq == 64 || a.dq == 128) && (a.dv == 64 || a.dv == 128);
   const bool aligned = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) & 15) == 0;
   return !a.f32 && wide && aligned && a.heads / a.kv_heads <= 128 && a.scale > 0.f &&
-         (long long)row_tiles(a) * a.b * a.kv_heads * 64 <= 0x7fffffffLL;
+         (long long)row_tiles(a) * a.b * a.kv_heads * UGB_MASKED_SPLITS <= 0x7fffffffLL;
 }
 
-void ugb_masked_tc_shape(const ugb_device *dev, const ugb_masked_attention_args &a, long long *ctas, long long *slots) {
-  *ctas = (long long)row_tiles(a) * a.b * a.kv_heads;
-  *slots = (long long)(groups_of(a) == 1 && a.dq + a.dv == 128 ? 2 : 1) * dev->sm_count;
+void ugb_masked_tc_shape(const ugb_device *dev, const ugb_masked_attention_args &a, long long *items, long long *slots, int *parts, int *positions) {
+  *items = (long long)row_tiles(a) * a.b * a.kv_heads;
+  *parts = groups_of(a) == 0 ? 4 : 1;
+  *positions = per_group(a) * std::max(1, groups_of(a)) / (a.heads / a.kv_heads);
+  *slots = (long long)(groups_of(a) <= 1 && a.dq + a.dv == 128 ? 2 : 1) * dev->sm_count;
 }
 
 int32_t ugb_masked_tc_launch(ugb_device *dev, const ugb_masked_attention_args &a, const ugb_masked_params &m) {
