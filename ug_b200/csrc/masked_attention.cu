@@ -1,7 +1,7 @@
 // Attention of new positions over a sliding window and the first positions of a cache, or over the cache and their ancestors in a
 // tree (ugb_window_attend, ugb_tree_attend; see masked_attention.cuh).
 //
-//   masked_attention_tc_kernel        (masked_attention_tc.cu) bf16 heads of 64 or 128 values
+//   masked_attention_tc_kernel        (masked_attention_tc.cu) bf16 heads of up to 128 values
 //   masked_attention_generic_kernel   f32, other heads, unaligned buffers: plain FFMA over tiles of 64 keys
 //   masked_combine_kernel             joins the slices of the keys that ran as separate CTAs
 //

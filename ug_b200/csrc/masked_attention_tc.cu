@@ -1,4 +1,5 @@
-// Attention over a window or a tree on the 5th-generation tensor cores (see masked_attention.cuh), bf16 heads of 64 or 128 values.
+// Attention over a window or a tree on the 5th-generation tensor cores (see masked_attention.cuh), bf16 heads of up to 128 values: DQ and DV are 64 or 128,
+// what a head lacks of them is filled with zeros by TMA and cut off by it.
 //
 // One item = up to RT x 128 rows of a (sequence, key / value head) and a slice of the keys they see, in tiles of 128 keys (64 where 64 are enough); a row is
 // a query position of one head of the group, so that keys and values are read once for all heads that share them:
@@ -14,6 +15,10 @@
 // Grid: one CTA per item; a CTA that is done takes over the item of one that has not started (cluster launch control), so that its set-up and its
 // TMEM are shared by many and long and short items even out.  Every wait on an mbarrier is bounded.
 //
+// What it is bound by, at two groups of 128-wide heads: a tile of 128 keys takes 4000 cycles, of which its products' reads of shared memory are 3000 and the
+// two groups' exponentials 2048; of the rest of a softmax warp's chain, waits, stores and fences are 1400.  4 x 2048 positions over a window of 1024, 32
+// heads on 8: 198 us, 710 TF/s (204 without packed arithmetic and three-way maxima, 226 without the registers of the first warpgroup, 260 with the scores
+// taken from the tensor memory twice, 219 with a quarter of the exponentials on the FP32 pipe one by one, 202 in pairs).
 // Tiles of 128 keys and not 64: the waits, fences and stores of a tile cost a softmax warp 1000 cycles whatever its size, the exponentials of 64 keys
 // 950 to 1600; and the products read Q and P from shared memory once per 128 keys.
 #include <cuda_bf16.h>
@@ -37,7 +42,8 @@ constexpr int P_BYTES = 2 * BLOCK;                         // 128 rows x 128 key
 // RT 0: up to 32 rows, spread over the four warps of one group.
 template <int DQ, int DV, int RT0> struct Shape {
   static constexpr int RT = RT0 ? RT0 : 1;
-  static constexpr int THREADS = 64 + 128 * RT;
+  // Two groups: the softmax warps are two whole warpgroups, which take registers over from the first one (two of its warps have no part).
+  static constexpr int FIRST = RT == 2 ? 4 : 2, THREADS = 32 * FIRST + 128 * RT;    // FIRST: softmax warp
   static constexpr int Q_BYTES = DQ / CB * BLOCK, STAGE = (DQ > DV ? DQ : DV) / CB * BLOCK;     // a stage holds a tile of keys or of values
   static constexpr int O_COL = RT * KEYS;                  // TMEM: S [RT][128], then O [RT][DV]
   static constexpr int TMEM_USED = O_COL + RT * DV, TMEM_COLS = TMEM_USED <= 256 ? 256 : 512;
@@ -60,6 +66,29 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// Two values at a time, and three: the softmax warps are bound by the instructions they issue.
+struct Two { unsigned long long v; };
+__device__ __forceinline__ Two two(float x, float y) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void apart(Two a, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -204,6 +233,9 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
   const uint32_t tmem = *tmem_slot;
 
   // The ring's order: K(0), then K(j + 1), V(j) for every tile j, and V of the last one: the order in which the products are issued.
+  if (warp < Sh::FIRST) {
+  // of 168 registers per thread at the launch: 4 x 96 + 8 x 200 <= 12 x 168
+  if constexpr (RT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer --
     if (elect_one()) {
@@ -328,12 +360,14 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
         if (!alive) break;
       }
     }
+  }
   } else {
     // -------------------------------------------------------------- softmax warps --
-    const int a = (warp - 2) / 4, quad = warp & 3, row = quad * 32 + lane;              // TMEM lane = row of the group
+    if constexpr (RT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const int a = (warp - Sh::FIRST) / 4, quad = warp & 3, row = quad * 32 + lane;              // TMEM lane = row of the group
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16), s_base = lane_base + (uint32_t)(a * KEYS), o_base = lane_base + (uint32_t)(Sh::O_COL + a * DV);
     uint8_t *const p_group = p_s + a * P_BYTES, *const prow = p_group + row * 128;
-    const bool leader = threadIdx.x == 64 + a * 128;       // issues the group's stores
+    const bool leader = threadIdx.x == 32 * Sh::FIRST + a * 128;     // issues the group's stores
     bool alive = true;
     int g0 = 0;                                            // stages of the CTA so far
     uint32_t n_s = 0, n_o = 0;                             // S and O products of this group so far
@@ -347,7 +381,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
       if (idx < 0) break;
       const Item it = item_of<RT, TREE>(idx, p);
       if (!it.valid) {
-        if (it.pos != -1 && threadIdx.x == 64) raise_invalid(status, it.s);
+        if (it.pos != -1 && leader) raise_invalid(status, it.s);
         const int r = it.row0 + a * p.per_group + (SPREAD ? lane : row);
         if (p.m.part_ml && it.slice == 0 && r < p.m.rows && (!SPREAD || quad == 0) && (SPREAD || row < p.per_group))
           p.m.part_ml[((size_t)it.s * p.m.kv_heads + it.kvh) * p.m.rows + r] = make_float2(NAN, 0.f);       // for the combine kernel: to be left as it is
@@ -369,7 +403,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
             bad |= x < -1 || x >= j;
           }
           bad = group_or(1 + a, bad);
-          if (bad && threadIdx.x == 64) raise_invalid(status, it.s);
+          if (bad && leader) raise_invalid(status, it.s);
           if (!bad)
             for (int j = i; j >= 0; j = up[a][j]) (j < 64 ? nodes0 : nodes1) |= 1ull << (j & 63);
         }
@@ -486,7 +520,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
           }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < KEYS; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(f[e]));
+          for (int e = 0; e < KEYS / 2; ++e) mx[e & 3] = max3(mx[e & 3], __uint_as_float(f[2 * e]), __uint_as_float(f[2 * e + 1]));
           const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;        // sc > 0
           const bool grow = top > m_ref + 8.f;
           float alpha = 1.f;
@@ -496,16 +530,21 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
             l *= alpha;
           }
           const float neg = m_ref == -INFINITY ? 0.f : -m_ref;          // a row may see nothing of the tiles so far
-          float l4[4] = {0.f, 0.f, 0.f, 0.f};
+          const Two sc2 = two(sc, sc), neg2 = two(neg, neg);
+          Two sum[2] = {two(0.f, 0.f), two(0.f, 0.f)};
 #pragma unroll
           for (int e = 0; e < KEYS / 2; ++e) {
-            const float x = ex2(fmaf(__uint_as_float(f[2 * e]), sc, neg)), y = ex2(fmaf(__uint_as_float(f[2 * e + 1]), sc, neg));
-            l4[2 * e & 3] += x;
-            l4[(2 * e + 1) & 3] += y;
+            float x, y;
+            apart(fma2(two(__uint_as_float(f[2 * e]), __uint_as_float(f[2 * e + 1])), sc2, neg2), x, y);
+            x = ex2(x);
+            y = ex2(y);
+            sum[e & 1] = add2(sum[e & 1], two(x, y));
             const __nv_bfloat162 t = __floats2bfloat162_rn(x, y);
             f[e] = *reinterpret_cast<const uint32_t *>(&t);
           }
-          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+          float x, y;
+          apart(add2(sum[0], sum[1]), x, y);
+          l += x + y;
           // the product before has retired: its probabilities may be overwritten, and O is at rest
           if (j > 0) {
             if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&o_full[a]), n_o & 1u, abort_flag, status, 0x6d))) { alive = false; break; }
@@ -609,7 +648,8 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
             if (write) {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
-                *reinterpret_cast<uint4 *>(p.m.part_o + (pair * (DV / 4) + (c + e) / 4) * p.m.rows + out_row) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                if (c + e < p.m.dv)
+                  *reinterpret_cast<uint4 *>(p.m.part_o + (pair * (p.m.dv / 4) + (c + e) / 4) * p.m.rows + out_row) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
           }
         }
@@ -650,7 +690,7 @@ int32_t launch(ugb_device *dev, const ugb_masked_attention_args &a, const Params
     const uint32_t box[4] = {(uint32_t)CB, 1, 64, 1};
     return ugb_tc_encode_bf16(dev, m, (const __nv_bfloat16 *)base, 4, dims, strides, box);
   };
-  if ((rc = q_map(&tmQ, a.q, DQ)) || (rc = q_map(&tmO, a.out, DV)) || (rc = kv_map(&tmK, a.k, DQ)) || (rc = kv_map(&tmV, a.v, DV))) return rc;
+  if ((rc = q_map(&tmQ, a.q, a.dq)) || (rc = q_map(&tmO, a.out, a.dv)) || (rc = kv_map(&tmK, a.k, a.dq)) || (rc = kv_map(&tmV, a.v, a.dv))) return rc;
   masked_attention_tc_kernel<DQ, DV, RT0, TREE><<<(unsigned)((long long)p.row_tiles * p.pairs * p.m.splits), Sh::THREADS, Sh::SMEM_BYTES, dev->stream>>>(tmQ, tmK, tmV, tmO, p);
   return ugb_after_launch(dev, "masked_attention_tc_kernel");
 }
@@ -678,7 +718,7 @@ template <int DQ, int DV> int32_t launch_any(ugb_device *dev, const ugb_masked_a
 }  // namespace
 
 bool ugb_masked_tc_takes(const ugb_masked_attention_args &a) {
-  const bool wide = (a.dq == 64 || a.dq == 128) && (a.dv == 64 || a.dv == 128);
+  const bool wide = a.dq <= 128 && a.dv <= 128;
   const bool aligned = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) & 15) == 0;
   return !a.f32 && wide && aligned && a.heads / a.kv_heads <= 128 && a.scale > 0.f &&
          (long long)row_tiles(a) * a.b * a.kv_heads * UGB_MASKED_SPLITS <= 0x7fffffffLL;
@@ -688,13 +728,13 @@ void ugb_masked_tc_shape(const ugb_device *dev, const ugb_masked_attention_args 
   *items = (long long)row_tiles(a) * a.b * a.kv_heads;
   *parts = groups_of(a) == 0 ? 4 : 1;
   *positions = per_group(a) * std::max(1, groups_of(a)) / (a.heads / a.kv_heads);
-  *slots = (long long)(groups_of(a) <= 1 && a.dq + a.dv == 128 ? 2 : 1) * dev->sm_count;
+  *slots = (long long)(groups_of(a) <= 1 && a.dq <= 64 && a.dv <= 64 ? 2 : 1) * dev->sm_count;
 }
 
 int32_t ugb_masked_tc_launch(ugb_device *dev, const ugb_masked_attention_args &a, const ugb_masked_params &m) {
   Params p;
   p.m = m;
   p.pairs = a.b * a.kv_heads; p.row_tiles = row_tiles(a); p.per_group = per_group(a);
-  if (a.dq == 64) return a.dv == 64 ? launch_any<64, 64>(dev, a, p) : launch_any<64, 128>(dev, a, p);
-  return a.dv == 64 ? launch_any<128, 64>(dev, a, p) : launch_any<128, 128>(dev, a, p);
+  if (a.dq <= 64) return a.dv <= 64 ? launch_any<64, 64>(dev, a, p) : launch_any<64, 128>(dev, a, p);
+  return a.dv <= 64 ? launch_any<128, 64>(dev, a, p) : launch_any<128, 128>(dev, a, p);
 }
