@@ -571,7 +571,7 @@ template <typename T>
 int32_t launch(ugb_device *dev, const Params &p, int size) {
   static bool attr_set[64] = {};
   if (!attr_set[dev->ordinal & 63]) {
-    UGB_CUDA(dev, cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, UGB_SAMPLE_VOCAB_MAX / CLUSTER_MAX * (int)sizeof(T)));
+    UGB_CUDA(dev, cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 161 * 1024));
     attr_set[dev->ordinal & 63] = true;
   }
   const cudaError_t e = ugb_launch_cluster(sample_kernel<T>, dim3((unsigned)(p.rows * size)), dim3(THREADS), (size_t)p.chunk * sizeof(T), dev->stream, false, size, p, size);
@@ -586,9 +586,12 @@ int32_t ugb_sample_rows(ugb_device *dev, const ugb_sample_args &a) {
   Params p;
   p.logits = a.logits; p.temperature = a.temperature; p.top_p = a.top_p; p.min_p = a.min_p; p.u = a.u; p.top_k = a.top_k; p.tokens = a.tokens;
   p.prob = a.prob; p.rows = a.rows; p.vocab = a.vocab; p.ld = a.ld; p.status = dev->status_dev;
-  // CTAs of a row: so many that the GPU is full, and that a row leaves room for three CTAs on an SM
+  // CTAs of a row: 4 where rows alone do not fill the GPU or are long, so that two and more share an SM; 8 only where 4 cannot hold it, since every exchange
+  // in a cluster costs more the larger it is (1 x 32000 in 1 / 2 / 4 / 8 CTAs 18.5 / 16.4 / 15.0 / 18.4 us, 64 x 32000 48.5 / 32.1 / 28.8 / 49.5, 256 x 131072
+  // bf16 in 2 / 4 / 8 411 / 309 / 461)
   int size = 1;
-  while (size < CLUSTER_MAX && ((long long)a.rows * size < dev->sm_count || (a.vocab + size - 1) / size > (a.bf16 ? 32768 : 16384))) size *= 2;
+  while (size < 4 && ((long long)a.rows * size < 4LL * dev->sm_count || (a.vocab + size - 1) / size > 8192)) size *= 2;
+  if ((long long)(a.vocab / size) * (a.bf16 ? 2 : 4) > 160 * 1024) size = CLUSTER_MAX;
   p.chunk = ((a.vocab + size - 1) / size + 15) / 16 * 16;
   p.seg = (p.chunk + THREADS - 1) / THREADS | 1;
   return a.bf16 ? launch<__nv_bfloat16>(dev, p, size) : launch<float>(dev, p, size);
