@@ -118,6 +118,18 @@ def test_tree(dev, bf16, dq, dv, heads, kv, t, t_max, pos):
     Call(dev, bf16, len(pos), t, heads, kv, dq, dv, t_max, pos, parents=parents).run().check()
 
 
+@pytest.mark.parametrize("bf16,dq,dv,share,t,kind", [(True, 64, 64, 1, 1, "window"), (True, 64, 64, 8, 1, "window"), (True, 64, 64, 32, 1, "tree"), (True, 128, 128, 4, 1, "window"),
+                                                     (True, 128, 64, 5, 6, "tree"), (True, 40, 96, 3, 10, "window"), (False, 64, 64, 4, 1, "window"), (True, 128, 128, 8, 4, "tree"),
+                                                     (True, 64, 64, 11, 3, "window")])
+def test_many_sequences_over_long_caches(dev, bf16, dq, dv, share, t, kind):
+    """Few rows each of more sequences than the GPU has SMs, over thousands of keys: lengths of one key to all, first positions and windows that meet and do not."""
+    b, kv, t_max, r = 75, 2, 2304, synth.rng(77)
+    pos = [int(p) for p in r.integers(0, t_max - t, b)]
+    pos[3], pos[10], pos[11], pos[40], pos[41] = 0, -1, t_max - t, 127, 128
+    parents = np.array([tree(80 + s, t) for s in range(b)]) if kind == "tree" else None
+    Call(dev, bf16, b, t, share * kv, kv, dq, dv, t_max, pos, parents=parents, sinks=70, window=2100).run().check()
+
+
 @pytest.mark.parametrize("bf16", [False, True])
 @pytest.mark.parametrize("kind", ["chain", "star", "roots"])
 def test_shapes_of_trees(dev, bf16, kind):

@@ -295,7 +295,7 @@ template <typename T, bool COPIES> cudaError_t launch_rows(bool tree, int rm, di
 int slices(long long items, long long slots, int tiles, int parts, int start) {
   int best = 1;
   double least = 1e30;
-  for (int s = 1; s * parts <= UGB_MASKED_SPLITS && (s == 1 || tiles >= 2 * s); ++s) {
+  for (int s = 1; s * parts <= UGB_MASKED_SPLITS && (s == 1 || (tiles >= 2 * s && items * s <= 0x7fffffffLL)); ++s) {
     const long long rounds = (items * s + slots - 1) / slots;
     const double all = (double)rounds * ((tiles + s - 1) / s + (s > 1 ? 2 * start : start)) + (s > 1 ? 0.25 * s * (1 + parts) : 0.0);
     if (all < least) { least = all; best = s; }
@@ -314,7 +314,7 @@ int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a
   p.heads = a.heads; p.kv_heads = a.kv_heads; p.share = a.heads / a.kv_heads; p.rows = a.t * p.share; p.dq = a.dq; p.dv = a.dv;
   p.scale = a.scale * LOG2E; p.out_scale = a.out_scale; p.part_o = nullptr; p.part_ml = nullptr; p.status = dev->status_dev;
   const int pairs = a.b * a.kv_heads;
-  const bool tc = ugb_masked_tc_takes(a);
+  const bool tc = ugb_masked_tc_takes(dev, a);
   const int rm = p.rows <= 16 ? 1 : 4, row_tiles = (p.rows + 16 * rm - 1) / (16 * rm);
   long long items = (long long)row_tiles * pairs, slots = 2LL * dev->sm_count;
   int parts = 1, positions = 16 * rm / p.share + 1;

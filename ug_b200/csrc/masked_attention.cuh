@@ -60,7 +60,7 @@ template <bool TREE> __device__ __forceinline__ Span span_of(const ugb_mask &m, 
 
 // The tensor-core kernel (masked_attention_tc.cu).  Whether it takes a call; how many items a slice of the keys has, how many run at a time, into
 // how many parts each leaves its slice's result and how many query positions it has; its launch.
-bool ugb_masked_tc_takes(const ugb_masked_attention_args &a);
+bool ugb_masked_tc_takes(const ugb_device *dev, const ugb_masked_attention_args &a);
 void ugb_masked_tc_shape(const ugb_device *dev, const ugb_masked_attention_args &a, long long *items, long long *slots, int *parts, int *positions);
 int32_t ugb_masked_tc_launch(ugb_device *dev, const ugb_masked_attention_args &a, const ugb_masked_params &p);
 

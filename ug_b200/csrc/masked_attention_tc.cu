@@ -695,46 +695,53 @@ int32_t launch(ugb_device *dev, const ugb_masked_attention_args &a, const Params
   return ugb_after_launch(dev, "masked_attention_tc_kernel");
 }
 
-// Groups of 128 rows in a CTA; 0: up to 32 rows in all.
-int groups_of(const ugb_masked_attention_args &a) {
+// Groups of 128 rows in a CTA; 0: up to 32 rows in all, spread, where the sequences alone fill the GPU and the keys may be so many that HBM is the bound: only
+// then is it worth joining the quarters (one position each of 64 sequences, 32 heads on 8 of 128: 1000 keys 57.8 us against 56.4 in one group, 4000 keys
+// 158 against 182; of one sequence, 32 on 4 of 64, 2000 keys 18.4 against 16.4, 16000 keys 36.9 against 30.2).
+int groups_of(const ugb_masked_attention_args &a, int sms) {
   const int share = a.heads / a.kv_heads;
-  return a.t * share <= 32 ? 0 : a.t > 128 / share ? 2 : 1;
+  const long long reach = a.parents ? a.t_max : std::min<long long>(a.t_max, (long long)a.window + a.t + a.sinks);
+  return a.t * share <= 32 && reach >= 2048 && (long long)a.b * a.kv_heads >= sms ? 0 : a.t > 128 / share ? 2 : 1;
 }
-int per_group(const ugb_masked_attention_args &a) {
+int per_group(const ugb_masked_attention_args &a, int sms) {
   const int share = a.heads / a.kv_heads;
-  return groups_of(a) == 0 ? share * a.t : share * (128 / share);
+  return groups_of(a, sms) == 0 ? share * a.t : share * (128 / share);
 }
-int row_tiles(const ugb_masked_attention_args &a) {
-  const int per = per_group(a) * std::max(1, groups_of(a));
+int row_tiles(const ugb_masked_attention_args &a, int sms) {
+  const int per = per_group(a, sms) * std::max(1, groups_of(a, sms));
   return (a.t * (a.heads / a.kv_heads) + per - 1) / per;
 }
 
 template <int DQ, int DV> int32_t launch_any(ugb_device *dev, const ugb_masked_attention_args &a, const Params &p) {
-  if (groups_of(a) == 0) return a.parents ? launch<DQ, DV, 0, true>(dev, a, p) : launch<DQ, DV, 0, false>(dev, a, p);
-  if (groups_of(a) == 1) return a.parents ? launch<DQ, DV, 1, true>(dev, a, p) : launch<DQ, DV, 1, false>(dev, a, p);
+  const int sms = dev->sm_count;
+  if (groups_of(a, sms) == 0) return a.parents ? launch<DQ, DV, 0, true>(dev, a, p) : launch<DQ, DV, 0, false>(dev, a, p);
+  if (groups_of(a, sms) == 1) return a.parents ? launch<DQ, DV, 1, true>(dev, a, p) : launch<DQ, DV, 1, false>(dev, a, p);
   return a.parents ? launch<DQ, DV, 2, true>(dev, a, p) : launch<DQ, DV, 2, false>(dev, a, p);
 }
 
 }  // namespace
 
-bool ugb_masked_tc_takes(const ugb_masked_attention_args &a) {
+bool ugb_masked_tc_takes(const ugb_device *dev, const ugb_masked_attention_args &a) {
+  const int sms = dev->sm_count;
   const bool wide = a.dq <= 128 && a.dv <= 128;
   const bool aligned = (((uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v | (uintptr_t)a.out) & 15) == 0;
   return !a.f32 && wide && aligned && a.heads / a.kv_heads <= 128 && a.scale > 0.f &&
-         (long long)row_tiles(a) * a.b * a.kv_heads * UGB_MASKED_SPLITS <= 0x7fffffffLL;
+         (long long)row_tiles(a, sms) * a.b * a.kv_heads <= 0x7fffffffLL;
 }
 
 void ugb_masked_tc_shape(const ugb_device *dev, const ugb_masked_attention_args &a, long long *items, long long *slots, int *parts, int *positions) {
-  *items = (long long)row_tiles(a) * a.b * a.kv_heads;
-  *parts = groups_of(a) == 0 ? 4 : 1;
-  *positions = per_group(a) * std::max(1, groups_of(a)) / (a.heads / a.kv_heads);
-  *slots = (long long)(groups_of(a) <= 1 && a.dq <= 64 && a.dv <= 64 ? 2 : 1) * dev->sm_count;
+  const int sms = dev->sm_count;
+  *items = (long long)row_tiles(a, sms) * a.b * a.kv_heads;
+  *parts = groups_of(a, sms) == 0 ? 4 : 1;
+  *positions = per_group(a, sms) * std::max(1, groups_of(a, sms)) / (a.heads / a.kv_heads);
+  *slots = (long long)(groups_of(a, sms) <= 1 && a.dq <= 64 && a.dv <= 64 ? 2 : 1) * dev->sm_count;
 }
 
 int32_t ugb_masked_tc_launch(ugb_device *dev, const ugb_masked_attention_args &a, const ugb_masked_params &m) {
+  const int sms = dev->sm_count;
   Params p;
   p.m = m;
-  p.pairs = a.b * a.kv_heads; p.row_tiles = row_tiles(a); p.per_group = per_group(a);
+  p.pairs = a.b * a.kv_heads; p.row_tiles = row_tiles(a, sms); p.per_group = per_group(a, sms);
   if (a.dq <= 64) return a.dv <= 64 ? launch_any<64, 64>(dev, a, p) : launch_any<64, 128>(dev, a, p);
   return a.dv <= 64 ? launch_any<128, 64>(dev, a, p) : launch_any<128, 128>(dev, a, p);
 }
