@@ -57,7 +57,7 @@ template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("c
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
 template <typename T, int RM, int NC, bool TREE, bool COPIES>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, NC == 1 ? 3 : 2)
 masked_attention_generic_kernel(Params p) {
   constexpr int TR = 16 * RM, PLD = KEYS + 4;
   extern __shared__ __align__(16) float gsm[];
@@ -316,7 +316,7 @@ int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a
   const int pairs = a.b * a.kv_heads;
   const bool tc = ugb_masked_tc_takes(dev, a);
   const int rm = p.rows <= 16 ? 1 : 4, row_tiles = (p.rows + 16 * rm - 1) / (16 * rm);
-  long long items = (long long)row_tiles * pairs, slots = 2LL * dev->sm_count;
+  long long items = (long long)row_tiles * pairs, slots = (a.dv <= 64 ? 3LL : 2LL) * dev->sm_count;
   int parts = 1, positions = 16 * rm / p.share + 1;
   if (tc) ugb_masked_tc_shape(dev, a, &items, &slots, &parts, &positions);
   // the most keys that the rows of an item can see: their positions are on the device
