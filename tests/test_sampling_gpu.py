@@ -218,6 +218,29 @@ def test_models_feed_the_sampled_tokens(dev):
         assert np.array_equal(m.logits(), other.logits())
 
 
+def test_llama_feeds_the_sampled_tokens(dev):
+    """The same of the Llama engine, through its captured step too."""
+    from ug_b200 import llama
+    cfg = llama.Config(hidden_size=256, intermediate_size=512, max_position_embeddings=128, num_attention_heads=4, num_key_value_heads=2, num_hidden_layers=2, vocab_size=512)
+    w, prompt = synth.llama_weights(cfg, 11), synth.tokens(15, (3, 7), 512)
+    m, other = (llama.Model.new(cfg, w, dev, 3, 64) for _ in range(2))
+    with pytest.raises(UgError):
+        m.sample(0.5)
+    m.prefill(prompt)
+    other.prefill(prompt)
+    for i in range(4):
+        u, x = synth.uniform(40 + i, (3,), 0, 1), m.logits()
+        m.sample(u, temperature=[1.5, 0.0, 0.7], top_k=100, min_p=0.01)
+        want = [choose(x[r], float(u[r]), [1.5, 0.0, float(np.float32(0.7))][r], 100, 1.0, float(np.float32(0.01)))[0] for r in range(3)]
+        assert m.next_tokens().tolist() == want
+        m.decode(1)
+        other.fwd(np.array(want, np.int32))
+        assert np.array_equal(m.logits(), other.logits())
+    m.close()
+    other.close()
+    assert lib.ugb_llama_sample(None, *[None] * 6) == 1 and lib.ugb_hybrid_sample(None, *[None] * 6) == 1
+
+
 def test_generate_with_random_numbers(dev):
     from ug_b200.generate import generate
     m = small_model(dev, 2)

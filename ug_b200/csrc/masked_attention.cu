@@ -291,11 +291,11 @@ template <typename T, bool COPIES> cudaError_t launch_rows(bool tree, int rm, di
 // Slices of the keys, for `items` CTAs' worth of work of `tiles` tiles of 64 keys each on `slots`: what is shortest, in tiles, for the CTA that has most to do,
 // where an item's start takes `start` tiles, twice that when its sums leave through memory, and joining them half a tile per slice (measured: 24 nodes
 // over 2000 positions in 4 / 6 / 8 / 12 slices 22.5 / 20.5 / 18.5 / 20.5 us, 64 nodes of 16 sequences over 8192 in 1 / 2 / 4 168 / 193 / 198 us, f32 in
-// 1 / 2 / 3 / 4, a block of 777, 135 / 121 / 118 / 125 us).
+// 1 / 2 / 3 / 4, a block of 777, 135 / 121 / 118 / 125 us).  No more items than 16 rounds of CTAs: their sums take memory.
 int slices(long long items, long long slots, int tiles, int parts, int start) {
   int best = 1;
   double least = 1e30;
-  for (int s = 1; s * parts <= UGB_MASKED_SPLITS && (s == 1 || (tiles >= 2 * s && items * s <= 0x7fffffffLL)); ++s) {
+  for (int s = 1; s * parts <= UGB_MASKED_SPLITS && (s == 1 || (tiles >= 2 * s && items * s <= 16 * slots)); ++s) {
     const long long rounds = (items * s + slots - 1) / slots;
     const double all = (double)rounds * ((tiles + s - 1) / s + (s > 1 ? 2 * start : start)) + (s > 1 ? 0.25 * s * (1 + parts) : 0.0);
     if (all < least) { least = all; best = s; }
