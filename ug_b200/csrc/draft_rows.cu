@@ -326,8 +326,11 @@ extern "C" int32_t ugb_tree_inputs(ugb_device *dev, const ugb_slice *pre, const 
   p.parents = (const int *)parents->ptr; p.q = q->ptr; p.k = kcache->ptr; p.v = vcache->ptr; p.t = (int)t; p.heads = (int)heads;
   p.kv_heads = (int)kv_heads; p.dim = (int)dim; p.vdim = (int)vdim; p.rot = (int)rot_dims; p.interleaved = interleaved != 0;
   p.norm = qk_norm != 0; p.eps = eps; p.t_max = (int)t_max; p.status = dev->status_dev;
-  // several nodes share the look at the tree where there are more than fill the GPU
-  const size_t fill = 4 * (size_t)dev->sm_count, per = (b * t + fill - 1) / fill < t ? (b * t + fill - 1) / fill : t;
+  // several nodes share the look at the tree where there are more than fill the GPU, and so many that all CTAs run at once (64 x 64 nodes of 48 heads in
+  // 640 CTAs 31.3 us, in the 512 that do 29.7)
+  const size_t fill = 4 * (size_t)dev->sm_count;
+  size_t per = 1;
+  while (per < t && b * ((t + per - 1) / per) > fill) ++per;
   const dim3 grid((unsigned)(b * ((t + per - 1) / per)));
   // rows start at multiples of 8 values: aligned buffers make every piece of 8 aligned (the tables' too, where rot % 16 == 0)
   const bool vec = aligned16(pre->ptr) && aligned16(q->ptr) && aligned16(kcache->ptr) && aligned16(vcache->ptr) && aligned16(cos_->ptr) && aligned16(sin_->ptr);
