@@ -104,7 +104,7 @@ masked_attention_generic_kernel(Params p) {
   for (int r = ty; r < TR; r += 16) {
     const int row = row0 + r;
     const T *x = q + (((size_t)s * p.mask.t + row / p.share) * p.heads + kvh * p.share + row % p.share) * dq;
-    for (int c = tx; c < dq; c += 16) qs[r * kld + c] = r < n_rows ? (float)x[c] : 0.f;
+    for (int c = tx; c < dq; c += 16) qs[r * kld + c] = r < n_rows ? (float)x[c] * p.scale : 0.f;
   }
   float m[RM], l[RM], o[RM][4 * NC];
   int at[RM];                                              // absolute position of a row's query
@@ -141,30 +141,36 @@ masked_attention_generic_kernel(Params p) {
           sc[i][j] = fmaf(a[i].w, b[j].w, sc[i][j]);
         }
     }
+    // a tile that every row sees whole, as most are, needs no mask
+    const int low = key_of(tile * KEYS), high = key_of(min(tile * KEYS + KEYS, n_keys) - 1);
+    const bool whole = tile * KEYS + KEYS <= n_keys && (TREE ? high < pos : high <= pos + i0 && (low > pos + i1 - p.mask.window || high < p.mask.sinks));
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int place = tile * KEYS + tx + 16 * j, key = key_of(place);
+          bool on;
+          if constexpr (TREE) {
+            const int node = key - pos;
+            on = node < 0 || (node < p.mask.t && (bits[(ty * RM + i) * 4 + (node >> 5)] >> (node & 31) & 1u));
+          } else {
+            on = key <= at[i] && (key > at[i] - p.mask.window || key < p.mask.sinks);
+          }
+          if (!(on && place < n_keys)) sc[i][j] = -INFINITY;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int place = tile * KEYS + tx + 16 * j, key = key_of(place);
-        bool on;
-        if constexpr (TREE) {
-          const int node = key - pos;
-          on = node < 0 || (node < p.mask.t && (bits[(ty * RM + i) * 4 + (node >> 5)] >> (node & 31) & 1u));
-        } else {
-          on = key <= at[i] && (key > at[i] - p.mask.window || key < p.mask.sinks);
-        }
-        sc[i][j] = on && place < n_keys ? sc[i][j] * p.scale : -INFINITY;
-        mx = fmaxf(mx, sc[i][j]);
-      }
+      float mx = fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3]));
 #pragma unroll
       for (int e = 8; e > 0; e >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, e));
       const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn;       // a row may see nothing of this tile
-      const float alpha = exp2f(m[i] - base);
+      const float alpha = ex2(m[i] - base);
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float w = exp2f(sc[i][j] - base);
+        const float w = ex2(sc[i][j] - base);
         sum += w;
         ps[(ty * RM + i) * PLD + tx + 16 * j] = w;
       }
@@ -227,6 +233,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 masked_combine_kernel(Params p, int pairs) {
   __shared__ T done[32][32 + 8];
+  ugb_pdl_wait();
   const int blocks = (p.rows + 31) / 32, pair = blockIdx.x / blocks, row0 = blockIdx.x % blocks * 32, n_rows = min(32, p.rows - row0);
   const int s = pair / p.kv_heads, kvh = pair % p.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = row0 + min(lane, n_rows - 1);
   const int c = min(blockIdx.y * 8 + warp, p.dv / 4 - 1);  // four columns; the last warps repeat one where dv ends
@@ -345,9 +352,10 @@ int32_t ugb_masked_attention(ugb_device *dev, const ugb_masked_attention_args &a
   if (rc == UGB_OK && sums > 1) {
     p.splits = sums;
     const dim3 rows((unsigned)(pairs * ((p.rows + 31) / 32)), (unsigned)((a.dv + 31) / 32));
-    if (a.f32) masked_combine_kernel<float><<<rows, 256, 0, dev->stream>>>(p, pairs);
-    else masked_combine_kernel<__nv_bfloat16><<<rows, 256, 0, dev->stream>>>(p, pairs);
-    rc = ugb_after_launch(dev, "masked_combine_kernel");
+    // a dependent launch: its way to the SMs runs beside the last items' end
+    const cudaError_t e = a.f32 ? ugb_launch(masked_combine_kernel<float>, rows, dim3(256), 0, dev->stream, true, p, pairs)
+                                : ugb_launch(masked_combine_kernel<__nv_bfloat16>, rows, dim3(256), 0, dev->stream, true, p, pairs);
+    rc = e != cudaSuccess ? ugb_fail(dev, UGB_ERR_CUDA, "launch of masked_combine_kernel failed: %s", cudaGetErrorString(e)) : ugb_after_launch(dev, "masked_combine_kernel");
   }
   if (work) cudaFreeAsync(work, dev->stream);
   return rc;

@@ -662,6 +662,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
   }
   tcgen05_fence_before();
   __syncthreads();
+  ugb_pdl_trigger();                                       // the combine kernel's CTAs may come and wait
   if (warp == 1) {
     tcgen05_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sh::TMEM_COLS) : "memory");
