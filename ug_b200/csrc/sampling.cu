@@ -175,18 +175,29 @@ __device__ int find_index(const Row<T> &r, Shared &sh, u64 target, u64 mine, u64
   __syncthreads();
   u64 low = before;
   for (int w = 0; w < warp; ++w) low += sh.warp_sum[w];
-  if (low + run - mine <= target && target < low + run) {  // one thread of one CTA
-    u64 sum = low + run - mine;
-    bool open = true;
-    r.each([&](int i, float v) {
-      const u64 w = weigh(v, r.base + i);
-      sum += w;
-      if (open && sum > target) {
-        open = false;
-        sh.slot[slot] = (u64)(r.base + i) + 1;
-        sh.slot[slot + 1] = w;
+  const uint32_t owner = __ballot_sync(0xffffffffu, low + run - mine <= target && target < low + run);
+  if (owner) {                                             // one thread of one CTA: its warp looks through its share together
+    const int src = __ffs(owner) - 1, first = (warp * 32 + src) * r.seg, end = min(r.len, first + r.seg);
+    u64 sum = __shfl_sync(0xffffffffu, low + run - mine, src);
+    for (int i0 = first; i0 < end; i0 += 32) {
+      const int i = i0 + lane;
+      const u64 w = i < end ? weigh(r.at(i), r.base + i) : 0;
+      u64 upto = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 n = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += n;
       }
-    });
+      const uint32_t over = __ballot_sync(0xffffffffu, sum + upto > target);
+      if (over) {
+        if (lane == __ffs(over) - 1) {
+          sh.slot[slot] = (u64)(r.base + i) + 1;
+          sh.slot[slot + 1] = w;
+        }
+        break;
+      }
+      sum += __shfl_sync(0xffffffffu, upto, 31);
+    }
   }
   cluster_sync_all();
   u64 at = 0, w = 0;
