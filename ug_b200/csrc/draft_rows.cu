@@ -11,25 +11,11 @@
 
 namespace {
 
-template <typename T> __device__ __forceinline__ float to_f32(T x) { return (float)x; }
-template <typename T> __device__ __forceinline__ T from_f32(float x);
-template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 // 8 consecutive values: one or two 16-byte accesses where VEC says that they are aligned
 template <bool VEC> __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&f)[8]) {
-  if constexpr (VEC) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  static_assert(!VEC, "aligned pieces are fetched as they lie");
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (float)p[i];
-  }
+  for (int i = 0; i < 8; ++i) f[i] = (float)p[i];
 }
 template <bool VEC> __device__ __forceinline__ void load8(const float *p, float (&f)[8]) {
   if constexpr (VEC) {
@@ -191,7 +177,7 @@ tree_inputs_kernel(InputParams p, int per) {
             if (d < p.rot) {
               const bool one = p.interleaved ? d % 2 == 0 : d < half;
               const int i = p.interleaved ? d / 2 : one ? d : d - half, other_d = p.interleaved ? d ^ 1 : one ? d + half : d - half;
-              const float a = to_f32(x[d]), b = to_f32(x[other_d]);
+              const float a = (float)x[d], b = (float)x[other_d];
               f[e] = one ? a * cs[i] - b * sn[i] : a * cs[i] + b * sn[i];
             }
           }
