@@ -253,7 +253,7 @@ masked_combine_kernel(Params p, int pairs) {
 #pragma unroll 8
   for (int z = 0; z < p.splits; ++z) {
     const float2 w = ml[z * n];
-    const bool some = w.x != -INFINITY;                    // otherwise nothing was seen, or written
+    const bool some = w.x != -INFINITY || w.y != 0.f;      // otherwise nothing was seen, or written; a sum of NaN under a maximum that ignores it goes on
     const float4 v = some ? o[z * step] : make_float4(0.f, 0.f, 0.f, 0.f);
     const float f = some ? ex2(w.x - m) : 0.f;
     l = fmaf(f, w.y, l);
