@@ -1,4 +1,4 @@
-"""Attention over a window or a tree where a row's softmax is undefined: a NaN in the query or in a key that is seen.
+"""Attention over a window or a tree where a row's softmax is undefined or takes in infinities: a NaN in the query or in a key that is seen, scores of -inf.
 What the definition gives does not depend on whether the keys ran in one piece, in slices, or spread over the warps of a CTA.  Tolerances are those of
 test_masked_attention_gpu.py."""
 import numpy as np
@@ -90,4 +90,24 @@ def test_rows_whose_only_keys_in_a_slice_are_not_numbers(dev, path, kind):
     undefined = np.zeros(c.values[0].shape[:3], bool)
     for s, m in enumerate(c.masks):
         undefined[s, :, :share] = m[:, t_max // 2:].any(1)[:, None]
+    compare(c, run(dev, c, path), undefined)
+
+
+@cases
+def test_scores_of_minus_infinity(dev, path, kind):
+    """Where all are, 0 / 0; where some are, these weigh nothing.  Every score of the others is finite."""
+    c = call_of(dev, path, kind, 400, full=True)
+    c.values[0][..., 5] = 1.0
+    share = c.values[0].shape[2] // c.values[1].shape[1]
+    undefined = np.zeros(c.values[0].shape[:3], bool)
+    for s, m in enumerate(c.masks):
+        seen = np.nonzero(m.any(0))[0]
+        if s == 0:                                         # everything that the first group sees
+            c.values[1][s, 0, seen, 5] = -np.inf
+            undefined[s, :, :share] = True
+        rest = seen[(seen % 3 == 1) & (seen < c.pos[s])]   # a third of the committed positions, of every group
+        c.values[1][s, :, rest, 5] = -np.inf
+        c.masks[s] = m & ~np.isin(np.arange(m.shape[1]), rest)
+    put(c, 0)
+    put(c, 1)
     compare(c, run(dev, c, path), undefined)

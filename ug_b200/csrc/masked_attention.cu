@@ -211,7 +211,7 @@ masked_attention_generic_kernel(Params p) {
     const int r = ty * RM + i, row = row0 + r;
     if (r >= n_rows) continue;
     if (p.splits == 1) {
-      const float f = l[i] > 0.f ? p.out_scale / l[i] : 0.f;
+      const float f = p.out_scale / l[i];                  // at least 1: a row sees itself; 0 where all its scores are -inf, which gives NaN
       T *out = (T *)p.out + (((size_t)s * p.mask.t + row / p.share) * p.heads + kvh * p.share + row % p.share) * dv;
 #pragma unroll
       for (int c = 0; c < 4 * NC; ++c)
@@ -259,7 +259,7 @@ masked_combine_kernel(Params p, int pairs) {
     l = fmaf(f, w.y, l);
     acc.x = fmaf(f, v.x, acc.x); acc.y = fmaf(f, v.y, acc.y); acc.z = fmaf(f, v.z, acc.z); acc.w = fmaf(f, v.w, acc.w);
   }
-  const float f = l > 0.f ? p.out_scale / l : 0.f;
+  const float f = p.out_scale / l;                         // as above
   T *d = &done[lane][4 * warp];
   d[0] = (T)(acc.x * f); d[1] = (T)(acc.y * f); d[2] = (T)(acc.z * f); d[3] = (T)(acc.w * f);
   __syncthreads();

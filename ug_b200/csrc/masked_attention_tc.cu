@@ -608,7 +608,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
       }
       if (!SPREAD && p.m.splits == 1) {
         // every item has tiles then; the probabilities' buffer takes the result, a block of 64 columns after the other
-        const float scale = l > 0.f ? p.m.out_scale / l : 0.f;
+        const float scale = p.m.out_scale / l;             // at least 1: a row sees itself; 0 where all its scores are -inf, which gives NaN
         if (busy) {
 #pragma unroll
           for (int c = 0; c < DV; c += 32) {
