@@ -742,8 +742,9 @@ UGB_API int32_t ugb_sample(ugb_device *dev, const ugb_slice *logits, const ugb_s
                            const ugb_slice *top_p, const ugb_slice *min_p, const ugb_slice *u, ugb_slice *tokens, ugb_slice *prob,
                            size_t rows, size_t vocab, size_t ld);
 /* The same over the logits of a model's last step or prompt: the tokens become what ugb_llama_decode(m, NULL, n) /
- * ugb_hybrid_decode feeds next and what UGB_*_NEXT_TOKENS reads, in place of the greedy ones.  A tensor-parallel rank
- * holds a part of the vocabulary only: UGB_ERR_UNSUPPORTED. */
+ * ugb_hybrid_decode feeds next and what UGB_*_NEXT_TOKENS reads, in place of the greedy ones.  UGB_ERR_INVALID where there are none: before the
+ * first step or prompt, and behind a reset to another position or a ugb_*_time_kernel.  A tensor-parallel rank holds a part of the
+ * vocabulary only: UGB_ERR_UNSUPPORTED. */
 UGB_API int32_t ugb_llama_sample(ugb_llama *m, const ugb_slice *temperature, const ugb_slice *top_k, const ugb_slice *top_p,
                                  const ugb_slice *min_p, const ugb_slice *u, ugb_slice *prob);
 UGB_API int32_t ugb_hybrid_sample(ugb_hybrid *m, const ugb_slice *temperature, const ugb_slice *top_k, const ugb_slice *top_p,

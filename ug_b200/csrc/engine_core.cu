@@ -52,6 +52,7 @@ int32_t engine_reset(ugb_engine *m, int32_t pos) {
   UGB_REQUIRE(dev, pos >= 0 && pos < m->t_max, UGB_ERR_INVALID, "reset position %d outside 0..%d", pos, m->t_max - 1);
   UGB_CUDA(dev, cudaMemcpyAsync(m->pos, &pos, 4, cudaMemcpyHostToDevice, dev->stream));
   UGB_CUDA(dev, cudaStreamSynchronize(dev->stream));
+  m->has_logits = m->has_logits && pos == m->host_pos;
   m->host_pos = pos;
   return UGB_OK;
 }
@@ -65,10 +66,9 @@ int32_t engine_decode(ugb_engine *m, const ugb_slice *tokens, int32_t n_steps) {
   UGB_CUDA(dev, cudaSetDevice(dev->ordinal));
   int32_t rc;
   if ((rc = m->before_step())) return rc;
-  if (tokens) {
-    UGB_SLICE(dev, tokens, UGB_I32, (size_t)m->batch);
-    UGB_CUDA(dev, cudaMemcpyAsync(m->next, tokens->ptr, (size_t)m->batch * 4, cudaMemcpyDeviceToDevice, dev->stream));
-  }
+  if (tokens) UGB_SLICE(dev, tokens, UGB_I32, (size_t)m->batch);
+  m->has_logits = false;
+  if (tokens) UGB_CUDA(dev, cudaMemcpyAsync(m->next, tokens->ptr, (size_t)m->batch * 4, cudaMemcpyDeviceToDevice, dev->stream));
   for (int s = 0; s < n_steps; ++s) {
     if (!m->warmed) {
       // first step runs eagerly: it sets kernel attributes, which must not happen inside a capture
@@ -94,6 +94,7 @@ int32_t engine_decode(ugb_engine *m, const ugb_slice *tokens, int32_t n_steps) {
     }
     m->host_pos++;
   }
+  m->has_logits = true;
   return UGB_OK;
 }
 
@@ -120,6 +121,7 @@ int32_t engine_prefill(ugb_engine *m, const ugb_slice *tokens, int32_t t, int32_
     }
     m->pf_logits_t = t;
   }
+  m->has_logits = false;
   const int *tok = (const int *)tokens->ptr;
   int tc = 0;
   for (int c0 = 0; c0 < t; c0 += tc) {
@@ -132,6 +134,7 @@ int32_t engine_prefill(ugb_engine *m, const ugb_slice *tokens, int32_t t, int32_
   UGB_CUDA(dev, cudaMemcpyAsync(m->pos, &last, 4, cudaMemcpyHostToDevice, dev->stream));
   if ((rc = m->enqueue_head(false))) return rc;
   m->host_pos += t;
+  m->has_logits = true;
   return UGB_OK;
 }
 
@@ -148,7 +151,7 @@ int32_t engine_read_rows(ugb_engine *m, const void *src, size_t rows, size_t col
 int32_t engine_sample(ugb_engine *m, const ugb_slice *temperature, const ugb_slice *top_k, const ugb_slice *top_p, const ugb_slice *min_p,
                       const ugb_slice *u, ugb_slice *prob) {
   ugb_device *dev = m->dev;
-  UGB_REQUIRE(dev, m->host_pos > 0, UGB_ERR_INVALID, "sample: no step or prompt has left logits");
+  UGB_REQUIRE(dev, m->has_logits, UGB_ERR_INVALID, "sample: no step or prompt has left logits");
   ugb_slice logits, tokens;
   logits.dev = tokens.dev = dev;
   logits.ptr = m->logits; logits.len = (size_t)m->batch * m->logits_ld; logits.dtype = UGB_F32;

@@ -16,6 +16,7 @@ struct ugb_engine {
   int host_pos = 0;
   float *logits = nullptr;        // [batch, logits_ld], the first `vl` columns are vocabulary entries
   int vl = 0, logits_ld = 0;
+  bool has_logits = false;        // they are those of position host_pos - 1: a step or a prompt ended there
   int pdl = 1;                    // programmatic dependent launch between the kernels of a step
   // graph of one step that reads `next` as its input tokens
   cudaGraphExec_t graph = nullptr;

@@ -771,6 +771,7 @@ int32_t ugb_hybrid_time_kernel(ugb_hybrid *m, int32_t which, int32_t t, int32_t 
   void *tok = nullptr;
   UGB_CUDA(dev, cudaMalloc(&tok, (size_t)m->batch * t * 4));
   UGB_CUDA(dev, cudaMemsetAsync(tok, 0, (size_t)m->batch * t * 4, dev->stream));
+  m->has_logits = false;
   cudaGraph_t g = nullptr;
   cudaGraphExec_t ge = nullptr;
   cudaError_t e = cudaStreamBeginCapture(dev->stream, cudaStreamCaptureModeThreadLocal);

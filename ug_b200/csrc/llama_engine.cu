@@ -1025,6 +1025,7 @@ int32_t ugb_llama_time_kernel(ugb_llama *m, int32_t which, int32_t iters, float 
   ugb_device *dev = m->dev;
   UGB_REQUIRE(dev, ms_per_pass && iters >= 1, UGB_ERR_INVALID, "ugb_llama_time_kernel: bad argument");
   UGB_REQUIRE(dev, m->host_pos >= 1, UGB_ERR_INVALID, "ugb_llama_time_kernel: the cache is empty");
+  m->has_logits = false;
   const ugb_llama_config &c = m->lc;
   const int H = c.hidden, AW = c.n_heads * c.head_dim;
   const float scale = powf((float)c.head_dim, -0.5f);

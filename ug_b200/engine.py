@@ -115,8 +115,8 @@ class EngineModel:
     def sample(self, u, temperature=None, top_k=None, top_p=None, min_p=None, prob=None):
         """Chooses the tokens of the last logits from the random numbers ``u`` (0 <= u < 1) instead of greedily: the next
         ``decode(1)`` feeds them and :meth:`next_tokens` reads them.  Every argument is one number for all sequences, an array of one
-        per sequence or a device Slice; ``prob``, a Slice, takes the tokens' probabilities.  Asynchronous; a value outside its
-        range is raised by the device's next ``synchronize``."""
+        per sequence or a device Slice; ``prob``, a Slice, takes the tokens' probabilities.  Refused before the first step or prompt and
+        behind a reset to another position.  Asynchronous; a value outside its range is raised by the device's next ``synchronize``."""
         rows = [self._per_row(x, d) for x, d in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32), (u, np.float32))]
         self.dev._check(self._fn("sample")(self._h, *[r._h if r is not None else None for r in rows], prob._h if prob is not None else None))
 
