@@ -11,9 +11,10 @@
 // (equal logits, a flat row), the next histogram divides the step by the logits' bits, until one logit or few tokens are left.
 //
 // Weights are summed as integers, in units of 2^-44 of the largest one: sums do not depend on their order, so that any number of CTAs and
-// any order of atomics gives the same token, and 2^18 tokens fit 63 bits.  A choice between neighbours hangs on sums that differ
-// by one weight: 32-bit exponentials (1e-7 of a sum) would draw another token of a flat row of 1e5 once in some hundred rows, 2^-45 each (4e-11) once
-// in 1e6 or more.  A token of less than 2^-45 of the best one's weight is never drawn.
+// any order of atomics gives the same token, and 2^18 tokens fit 63 bits.  A weight is off by half a unit and by 9e-15 of itself, a running sum by
+// less than 4e-14 of the total.  A choice between neighbours hangs on sums that differ by one weight: in a flat row of 1e5 a target lies that near a border
+// once in 1e8 rows (2 x 1e5 x 4e-14), near enough for 32-bit exponentials (1e-7) to draw another token once in 50.  A token of less than 2^-45 of the best
+// one's weight is never drawn.
 #include "sampling.cuh"
 
 #include <cuda_bf16.h>
@@ -32,7 +33,7 @@ typedef unsigned long long u64;
 constexpr int THREADS = 512, WARPS = THREADS / 32, CLUSTER_MAX = 8;
 constexpr int STEPS = 1024, RANKED = 256;
 constexpr float STEPS_PER_T = 32.0f;                       // 1024 steps reach to exp(-32) < 2^-45: what is beyond weighs nothing
-constexpr int POWERS = 256;
+constexpr int POWER_BITS = 9, POWERS = 1 << POWER_BITS;      // as many as threads
 constexpr float LOWEST_ABOVE = -3.4028232e38f;             // the second lowest value
 
 struct Params {
@@ -70,8 +71,8 @@ struct Shared {
   u64 pick[4];
 };
 
-// Weights, in units of 2^-44 of the best one's, by Tang's table method for the exponential: with t = 256 (x - best) log2(e) / T = n + f, |f| <= 1/2,
-// 2^(t / 256) is a power from the table, shifted, times 2^(f / 256) by its series to f^3 (1.4e-13 of the value).
+// Weights, in units of 2^-44 of the best one's, by Tang's table method for the exponential: with t = 512 (x - best) log2(e) / T = n + f, |f| <= 1/2,
+// 2^(t / 512) is a power from the table, shifted, times 2^(f / 512) by its series to f^3 (off by (ln 2 / 1024)^4 / 24 = 8.8e-15 of the value).
 struct Weights {
   float best, lowest;
   double best_d, k;
@@ -96,7 +97,7 @@ struct Weights {
     e = fma(e, f, 1.0);
     const double w = power[n & (POWERS - 1)];
     // + 2^8, whose last place is 2^-44
-    e = fma(__hiloint2double(__double2hiint(w) + ((n >> 8) << 20), __double2loint(w)), e, 256.0);
+    e = fma(__hiloint2double(__double2hiint(w) + ((n >> POWER_BITS) << 20), __double2loint(w)), e, 256.0);
     return ((u64)(uint32_t)(__double2hiint(e) - 0x40700000) << 32) | (uint32_t)__double2loint(e);
   }
 };
@@ -444,7 +445,8 @@ sample_kernel(Params p, int size) {
       best = fmaxf(best, f);
     }
   }
-  if (threadIdx.x < POWERS) sh.power[threadIdx.x] = exp2(threadIdx.x / (double)POWERS);
+  static_assert(POWERS == THREADS, "one power per thread");
+  sh.power[threadIdx.x] = exp2(threadIdx.x / (double)POWERS);
   uint32_t top = __reduce_max_sync(0xffffffffu, key_of(best));
   if ((threadIdx.x & 31) == 0) sh.warp_sum[threadIdx.x >> 5] = top;
   __syncthreads();
