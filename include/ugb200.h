@@ -736,7 +736,7 @@ UGB_API int32_t ugb_selective_step(ugb_device *dev, const ugb_slice *x, const ug
  * top_p, min_p, u F32 [rows], top_k I32 [rows], all but u null for 1, off, off, off; tokens I32 [rows]; prob
  * F32 [rows] or null: the chosen token's share of what stayed.  NaN and -inf are no candidates, a row of nothing
  * else gives token -1 and prob 0; +inf beats every finite logit.  Sums are exact integers: the same
- * row gives the same token in any batch.  A parameter outside its range (0 <= temperature <= 1e20, top_k >= 0,
+ * row gives the same token in any batch.  An output may take the place of a parameter, row by row.  A parameter outside its range (0 <= temperature <= 1e20, top_k >= 0,
  * top_p > 0, 0 <= min_p <= 1, 0 <= u < 1) is UGB_ERR_INVALID at the next ugb_sync, and its row is left as it was. */
 UGB_API int32_t ugb_sample(ugb_device *dev, const ugb_slice *logits, const ugb_slice *temperature, const ugb_slice *top_k,
                            const ugb_slice *top_p, const ugb_slice *min_p, const ugb_slice *u, ugb_slice *tokens, ugb_slice *prob,

@@ -303,8 +303,9 @@ extern "C" int32_t ugb_tree_inputs(ugb_device *dev, const ugb_slice *pre, const 
   UGB_SLICE(dev, sin_, UGB_F32, t_max * rot_dims / 2);
   UGB_SLICE(dev, pos, UGB_I32, b);
   UGB_SLICE(dev, parents, UGB_I32, b * t);
-  UGB_REQUIRE(dev, !ugb_overlap(pre, q) && !ugb_overlap(pre, kcache) && !ugb_overlap(pre, vcache) && !ugb_overlap(q, kcache) && !ugb_overlap(q, vcache) &&
-                       !ugb_overlap(kcache, vcache), UGB_ERR_INVALID, "tree_inputs: in place");
+  UGB_REQUIRE(dev, !ugb_overlap({ugb_used(q, b * t * heads * dim), ugb_used(kcache, b * kv_heads * t_max * dim), ugb_used(vcache, b * kv_heads * t_max * vdim)},
+                                {ugb_used(pre, b * t * ld), ugb_used(cos_, t_max * rot_dims / 2), ugb_used(sin_, t_max * rot_dims / 2), ugb_used(pos, b),
+                                 ugb_used(parents, b * t)}), UGB_ERR_INVALID, "tree_inputs: in place");
   if (b == 0 || t == 0) return UGB_OK;
   UGB_CUDA(dev, cudaSetDevice(dev->ordinal));
   InputParams p;
@@ -339,7 +340,8 @@ extern "C" int32_t ugb_cache_keep(ugb_device *dev, ugb_slice *k, ugb_slice *v, c
   UGB_SLICE(dev, pos, UGB_I32, b);
   UGB_SLICE(dev, path, UGB_I32, b * most);
   UGB_SLICE(dev, count, UGB_I32, b);
-  UGB_REQUIRE(dev, !ugb_overlap(k, v), UGB_ERR_INVALID, "cache_keep: the caches overlap");
+  UGB_REQUIRE(dev, !ugb_overlap({ugb_used(k, b * kv_heads * t_max * dq), ugb_used(v, b * kv_heads * t_max * dv)},
+                                {ugb_used(pos, b), ugb_used(path, b * most), ugb_used(count, b)}), UGB_ERR_INVALID, "cache_keep: the caches overlap, or one and the paths");
   if (b == 0 || most == 0) return UGB_OK;
   UGB_CUDA(dev, cudaSetDevice(dev->ordinal));
   KeepParams p;

@@ -378,7 +378,9 @@ int32_t attend(ugb_device *dev, const char *what, const ugb_slice *q, const ugb_
   UGB_SLICE(dev, v, q->dtype, b * kv_heads * t_max * dv);
   UGB_SLICE(dev, pos, UGB_I32, b);
   if (parents) UGB_SLICE(dev, parents, UGB_I32, b * t);
-  UGB_REQUIRE(dev, !ugb_overlap(out, q) && !ugb_overlap(out, k) && !ugb_overlap(out, v), UGB_ERR_INVALID, "%s: in place", what);
+  UGB_REQUIRE(dev, !ugb_overlap({ugb_used(out, b * t * heads * dv)}, {ugb_used(q, b * t * heads * dq), ugb_used(k, b * kv_heads * t_max * dq),
+                                                                       ugb_used(v, b * kv_heads * t_max * dv), ugb_used(pos, b), ugb_used(parents, b * t)}),
+              UGB_ERR_INVALID, "%s: in place", what);
   if (b == 0 || t == 0) return UGB_OK;
   UGB_CUDA(dev, cudaSetDevice(dev->ordinal));
   ugb_masked_attention_args a;

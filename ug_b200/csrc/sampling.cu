@@ -626,7 +626,12 @@ extern "C" int32_t ugb_sample(ugb_device *dev, const ugb_slice *logits, const ug
   UGB_SLICE(dev, u, UGB_F32, rows);
   UGB_SLICE(dev, tokens, UGB_I32, rows);
   if (prob) UGB_SLICE(dev, prob, UGB_F32, rows);
-  UGB_REQUIRE(dev, !ugb_overlap(logits, tokens) && !(prob && (ugb_overlap(logits, prob) || ugb_overlap(tokens, prob))), UGB_ERR_INVALID, "sample: in place");
+  const ugb_span chosen = ugb_used(tokens, rows), share = ugb_used(prob, rows);
+  UGB_REQUIRE(dev, !ugb_overlap({chosen, share}, {ugb_used(logits, rows ? (rows - 1) * ld + vocab : 0)}), UGB_ERR_INVALID, "sample: in place");
+  // a row reads its own setting before it writes in its place; a shifted one belongs to another row, which may come later
+  for (const ugb_slice *x : {temperature, top_k, top_p, min_p, u})
+    for (const ugb_span &y : {chosen, share})
+      UGB_REQUIRE(dev, !ugb_overlap(y, ugb_used(x, rows)) || y.from == (uintptr_t)x->ptr, UGB_ERR_INVALID, "sample: an output over other rows' settings");
   if (rows == 0) return UGB_OK;
   UGB_CUDA(dev, cudaSetDevice(dev->ordinal));
   ugb_sample_args a;

@@ -5,6 +5,7 @@
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/ugb200.h"
@@ -122,10 +123,21 @@ static inline int32_t ugb_check_slice(ugb_device *dev, const ugb_slice *s, int32
     if (rc__ != UGB_OK) return rc__;                                      \
   } while (0)
 
-// Whether two slices share memory.
-static inline bool ugb_overlap(const ugb_slice *a, const ugb_slice *b) {
-  const uintptr_t a0 = (uintptr_t)a->ptr, b0 = (uintptr_t)b->ptr, an = a->len * ugb_dtype_size(a->dtype), bn = b->len * ugb_dtype_size(b->dtype);
-  return an && bn && a0 < b0 + bn && b0 < a0 + an;
+// The memory of a slice's first n elements, which are what a call uses, and whether two share some.
+struct ugb_span { uintptr_t from, to; };
+static inline ugb_span ugb_used(const ugb_slice *s, size_t n) {
+  return s ? ugb_span{(uintptr_t)s->ptr, (uintptr_t)s->ptr + n * ugb_dtype_size(s->dtype)} : ugb_span{0, 0};
+}
+static inline bool ugb_overlap(const ugb_span &a, const ugb_span &b) { return a.from < a.to && b.from < b.to && a.from < b.to && b.from < a.to; }
+// Whether any output shares memory with an input or with another output.
+static inline bool ugb_overlap(std::initializer_list<ugb_span> outs, std::initializer_list<ugb_span> ins) {
+  for (const ugb_span *o = outs.begin(); o != outs.end(); ++o) {
+    for (const ugb_span &i : ins)
+      if (ugb_overlap(*o, i)) return true;
+    for (const ugb_span *x = outs.begin(); x != o; ++x)
+      if (ugb_overlap(*o, *x)) return true;
+  }
+  return false;
 }
 
 // ---- programmatic dependent launch ------------------------------------------
