@@ -16,3 +16,9 @@ def test_prompts_of_different_lengths(capsys):
     with pytest.raises(SystemExit):
         generate.main(["--model", "nowhere", "--prompt", "1,2", "--prompt", "1"])
     assert "one length" in capsys.readouterr().err
+
+
+def test_a_seed_below_zero(capsys):
+    with pytest.raises(SystemExit) as e:
+        generate.main(["--model", "nowhere", "--prompt", "1,2", "--seed", "-1"])
+    assert e.value.code == 2 and "seed" in capsys.readouterr().err
