@@ -22,3 +22,9 @@ def test_a_seed_below_zero(capsys):
     with pytest.raises(SystemExit) as e:
         generate.main(["--model", "nowhere", "--prompt", "1,2", "--seed", "-1"])
     assert e.value.code == 2 and "seed" in capsys.readouterr().err
+
+
+def test_a_share_that_vanishes_in_32_bits(capsys):
+    with pytest.raises(SystemExit) as e:
+        generate.main(["--model", "nowhere", "--prompt", "1,2", "--top-p", "1e-60"])
+    assert e.value.code == 2 and "top-p" in capsys.readouterr().err

@@ -66,7 +66,7 @@ def main(argv=None):
     a = ap.parse_args(argv)
     sampled = any(x is not None for x in (a.temperature, a.top_k, a.top_p, a.min_p, a.seed))
     for name, x, ok in (("temperature", a.temperature, lambda x: 0 <= x <= 1e20), ("top-k", a.top_k, lambda x: 0 <= x < 2 ** 31),
-                        ("top-p", a.top_p, lambda x: x > 0), ("min-p", a.min_p, lambda x: 0 <= x <= 1), ("seed", a.seed, lambda x: x >= 0)):
+                        ("top-p", a.top_p, lambda x: np.float32(x) > 0), ("min-p", a.min_p, lambda x: 0 <= x <= 1), ("seed", a.seed, lambda x: x >= 0)):
         if x is not None and not ok(x):
             ap.error(f"--{name} {x} is outside its range")
     from . import registry
