@@ -4,21 +4,18 @@ import pytest
 
 from test_draft_rows_gpu import I32
 from test_masked_attention_gpu import Call
-from test_masked_attention_undefined_gpu import PATHS, call_of, cases, run
+from test_masked_attention_undefined_gpu import PATHS, call_of, run
 from ug_b200 import UgError
 
 pytestmark = pytest.mark.gpu
 
 
-@cases
-@pytest.mark.parametrize("what", ["absent", "negative", "behind the cache", "tree"])
+@pytest.mark.parametrize("path,kind,what", [(p, k, w) for p in PATHS for k in ("window", "tree") for w in ("absent", "negative", "behind the cache", "tree") if w != "tree" or k == "tree"])
 def test_sequences_that_are_left_alone(dev, path, kind, what):
     """Their outputs stay as they were, whatever the scratch of the slices holds; the others are done."""
-    if what == "tree" and kind != "tree":
-        pytest.skip("a window has no tree")
     bf16, d, heads, kv, t, t_max, b, launches = PATHS[path]
     c = call_of(dev, path, kind, 500)
-    run(dev, c, path)                                      # scratch that has been used
+    run(dev, c, path)                                      # leaves its sums in the scratch
     two = b + 2                                            # in front of, between and behind the valid ones
     bad = [0, 2] if b == 1 else [0, b // 2, two - 1]
     pos, good = np.empty(two, np.int32), [s for s in range(two) if s not in bad]
