@@ -736,15 +736,16 @@ UGB_API int32_t ugb_selective_step(ugb_device *dev, const ugb_slice *x, const ug
  * top_p, min_p, u F32 [rows], top_k I32 [rows], all but u null for 1, off, off, off; tokens I32 [rows]; prob
  * F32 [rows] or null: the chosen token's share of what stayed.  NaN and -inf are no candidates, a row of nothing
  * else gives token -1 and prob 0; +inf beats every finite logit.  Sums are exact integers: the same
- * row gives the same token in any batch.  An output may take the place of a parameter, row by row.  A parameter outside its range (0 <= temperature <= 1e20, top_k >= 0,
- * top_p > 0, 0 <= min_p <= 1, 0 <= u < 1) is UGB_ERR_INVALID at the next ugb_sync, and its row is left as it was. */
+ * row gives the same token in any batch; weights are off by 2^-45 of the best one's and 9e-15 of themselves.  An output may take the
+ * place of a parameter, row by row.  A parameter outside its range (0 <= temperature <= 1e20, top_k >= 0, top_p > 0, 0 <= min_p <= 1,
+ * 0 <= u < 1) is UGB_ERR_INVALID at the next ugb_sync, and its row is left as it was. */
 UGB_API int32_t ugb_sample(ugb_device *dev, const ugb_slice *logits, const ugb_slice *temperature, const ugb_slice *top_k,
                            const ugb_slice *top_p, const ugb_slice *min_p, const ugb_slice *u, ugb_slice *tokens, ugb_slice *prob,
                            size_t rows, size_t vocab, size_t ld);
 /* The same over the logits of a model's last step or prompt: the tokens become what ugb_llama_decode(m, NULL, n) /
- * ugb_hybrid_decode feeds next and what UGB_*_NEXT_TOKENS reads, in place of the greedy ones.  UGB_ERR_INVALID where there are none: before the
- * first step or prompt, and behind a reset to another position or a ugb_*_time_kernel.  A tensor-parallel rank holds a part of the
- * vocabulary only: UGB_ERR_UNSUPPORTED. */
+ * ugb_hybrid_decode feeds next and what UGB_*_NEXT_TOKENS reads, in place of the greedy ones.  UGB_ERR_INVALID where there
+ * are none: before the first step or prompt, and behind a reset to another position or a ugb_*_time_kernel.  A
+ * tensor-parallel rank holds a part of the vocabulary only: UGB_ERR_UNSUPPORTED. */
 UGB_API int32_t ugb_llama_sample(ugb_llama *m, const ugb_slice *temperature, const ugb_slice *top_k, const ugb_slice *top_p,
                                  const ugb_slice *min_p, const ugb_slice *u, ugb_slice *prob);
 UGB_API int32_t ugb_hybrid_sample(ugb_hybrid *m, const ugb_slice *temperature, const ugb_slice *top_k, const ugb_slice *top_p,
@@ -763,7 +764,11 @@ UGB_API int32_t ugb_tree_inputs(ugb_device *dev, const ugb_slice *pre, const ugb
 /* Attention of t drafted nodes: query i attends the pos[s] committed positions, its node's ancestors and itself, whose keys and
  * values are in the cache rows above.  q T [b, t, heads, dq], k, v T [b, kv_heads, t_max, dq / dv], out T [b, t, heads, dv] times
  * out_scale; query head h reads head h / (heads / kv_heads); dq and dv multiples of 8 up to 256.  Cache rows behind the last node
- * may hold anything. */
+ * may hold anything.  A NaN in a query or in a key gives NaN in the rows that it belongs to or that see it, and so do scores that
+ * are all -inf; an infinite or NaN value, in a row that some query of the sequence sees, may give NaN to the other queries
+ * too (their weight for it is 0, and 0 x inf is NaN).  BF16 heads of up to 128 values, with aligned buffers and a scale above 0, run on
+ * the tensor cores, which take the weights in BF16 (off by 2^-8 of each at most); all else keeps them in 32 bits.  The number
+ * of slices of the keys follows from t_max, not from pos: a cache that is mostly empty costs some time and scratch. */
 UGB_API int32_t ugb_tree_attend(ugb_device *dev, const ugb_slice *q, const ugb_slice *k, const ugb_slice *v, const ugb_slice *pos,
                                 const ugb_slice *parents, ugb_slice *out, size_t b, size_t t, size_t heads, size_t kv_heads,
                                 size_t dq, size_t dv, size_t t_max, float scale, float out_scale);
@@ -776,7 +781,7 @@ UGB_API int32_t ugb_cache_keep(ugb_device *dev, ugb_slice *k, ugb_slice *v, cons
 /* Attention of t >= 1 new positions over a sliding window and the first positions: query i, at n = pos[s] + i, attends the
  * positions j <= n with j > n - window or j < sinks.  pos I32 [b], a position for every sequence, -1 as above; k and v
  * hold the new positions too (row pos[s] + i), and what no query of the block sees (rows ahead of the window, behind the
- * block) may hold anything.  q, out and head layouts as in ugb_tree_attend; any window >= 1, sinks >= 0.  Both
+ * block) may hold anything.  q, out, head layouts, types and what is not finite as in ugb_tree_attend; any window >= 1, sinks >= 0.  Both
  * take scratch for partial results from the device's stream-ordered pool for the duration of the call. */
 UGB_API int32_t ugb_window_attend(ugb_device *dev, const ugb_slice *q, const ugb_slice *k, const ugb_slice *v, const ugb_slice *pos,
                                   ugb_slice *out, size_t b, size_t t, size_t heads, size_t kv_heads, size_t dq, size_t dv,

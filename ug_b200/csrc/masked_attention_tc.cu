@@ -5,7 +5,8 @@
 // a query position of one head of the group, so that keys and values are read once for all heads that share them:
 //     warp 0        TMA producer: the rows' queries (one box: heads x positions), then key and value tiles into a ring
 //     warp 1        MMA issuer:   S = Q K^T of each 128 rows, O += P V, both accumulated in TMEM
-//     then 4 warps  softmax of 128 rows each (RT groups): one row per thread, no shuffles; P in bf16 through shared memory
+//     then 4 warps  softmax of 128 rows each (RT groups): one row per thread, no shuffles; P through shared memory in bf16, the type of V, as the product
+//                   takes both in one type (2^-8 of each probability, which the f32 sum does not have: the whole error is 1.4 times that of a result rounded once)
 // The scores of the next tile are formed as soon as this tile's are in registers, so that the softmax finds them ready; while one group's softmax runs, the
 // other's products do.  O stays in TMEM from the first tile to the last: it is rescaled only where a row's maximum has grown by more than 2^8 since
 // it was last (the probabilities are then up to 2^8, which costs bf16 no precision, and the sum is f32), which after the first tiles is hardly ever.
@@ -17,7 +18,7 @@
 //
 // What it is bound by, at two groups of 128-wide heads: a tile of 128 keys takes 4000 cycles, of which its products' reads of shared memory are 3000 and the
 // two groups' exponentials 2048; of the rest of a softmax warp's chain, waits, stores and fences are 1400.  4 x 2048 positions over a window of 1024, 32
-// heads on 8: 198 us, 710 TF/s (204 without packed arithmetic and three-way maxima, 226 without the registers of the first warpgroup, 260 with the scores
+// heads on 8: 198 to 205 us, 710 to 685 TF/s (beside 198 in one run: 204 without packed arithmetic and three-way maxima, 226 without the registers of the first warpgroup, 260 with the scores
 // taken from the tensor memory twice, 219 with a quarter of the exponentials on the FP32 pipe one by one, 202 in pairs).
 // Tiles of 128 keys and not 64: the waits, fences and stores of a tile cost a softmax warp 1000 cycles whatever its size, the exponentials of 64 keys
 // 950 to 1600; and the products read Q and P from shared memory once per 128 keys.

@@ -471,7 +471,7 @@ sample_kernel(Params p, int size) {
     prob = 1.0f;
   } else {
     if (best == INFINITY || best < LOWEST_ABOVE) {         // infinitely better than the others, or these are -inf: equal ones weigh the same
-      r.each([&](int i, float v) { x[i] = (T)(v == best ? 0.0f : -INFINITY); });          // every thread reads its own share only
+      r.each([&](int i, float v) { x[i] = (T)(v == best ? 0.0f : -INFINITY); });          // a thread's own share: other threads read it behind barriers
       best = 0.0f;
     }
     const Weights weights(best, temperature, sh.power);
@@ -600,8 +600,8 @@ int32_t ugb_sample_rows(ugb_device *dev, const ugb_sample_args &a) {
   p.logits = a.logits; p.temperature = a.temperature; p.top_p = a.top_p; p.min_p = a.min_p; p.u = a.u; p.top_k = a.top_k; p.tokens = a.tokens;
   p.prob = a.prob; p.rows = a.rows; p.vocab = a.vocab; p.ld = a.ld; p.status = dev->status_dev;
   // CTAs of a row: 4 where rows alone do not fill the GPU or are long, so that two and more share an SM; 8 only where 4 cannot hold it, since every exchange
-  // in a cluster costs more the larger it is (1 x 32000 in 1 / 2 / 4 / 8 CTAs 18.5 / 16.4 / 15.0 / 18.4 us, 64 x 32000 48.5 / 32.1 / 28.8 / 49.5, 256 x 131072
-  // bf16 in 2 / 4 / 8 411 / 309 / 461)
+  // in a cluster costs more the larger it is (1 x 32000 in 1 / 2 / 4 / 8 CTAs 20.9 / 16.4 / 15.6 / 19.8 us, 64 x 32000 44.4 / 30.6 / 28.0 / 49.6, 256 x 131072
+  // bf16 in 2 / 4 / 8 370 / 284 / 450)
   int size = 1;
   while (size < 4 && ((long long)a.rows * size < 4LL * dev->sm_count || (a.vocab + size - 1) / size > 8192)) size *= 2;
   if ((long long)(a.vocab / size) * (a.bf16 ? 2 : 4) > 160 * 1024) size = CLUSTER_MAX;
