@@ -764,9 +764,8 @@ UGB_API int32_t ugb_tree_inputs(ugb_device *dev, const ugb_slice *pre, const ugb
 /* Attention of t drafted nodes: query i attends the pos[s] committed positions, its node's ancestors and itself, whose keys and
  * values are in the cache rows above.  q T [b, t, heads, dq], k, v T [b, kv_heads, t_max, dq / dv], out T [b, t, heads, dv] times
  * out_scale; query head h reads head h / (heads / kv_heads); dq and dv multiples of 8 up to 256.  Cache rows behind the last node
- * may hold anything.  A NaN in a query or in a key gives NaN in the rows that it belongs to or that see it, and so do scores that
- * are all -inf; an infinite or NaN value, in a row that some query of the sequence sees, may give NaN to the other queries
- * too (their weight for it is 0, and 0 x inf is NaN).  BF16 heads of up to 128 values, with aligned buffers and a scale above 0, run on
+ * may hold anything, and so may what a query does not see of the others: a NaN or an infinite value reaches the queries that see it and no
+ * other.  Scores that are all -inf give NaN.  BF16 heads of up to 128 values, with aligned buffers and a scale above 0, run on
  * the tensor cores, which take the weights in BF16 (off by 2^-8 of each at most); all else keeps them in 32 bits.  The number
  * of slices of the keys follows from t_max, not from pos: a cache that is mostly empty costs some time and scratch. */
 UGB_API int32_t ugb_tree_attend(ugb_device *dev, const ugb_slice *q, const ugb_slice *k, const ugb_slice *v, const ugb_slice *pos,

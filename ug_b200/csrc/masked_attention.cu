@@ -11,6 +11,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -48,7 +49,8 @@ template <bool TREE> __device__ __forceinline__ bool check_sequence(const ugb_ma
 // that the rows see form one list, without the gap between the first ones and the window, cut into tiles of 64.
 // Shared memory, all f32: queries [16 RM][dq + 4], keys [64][dq + 4], values [64][dv + 4], probabilities [16 RM][64 + 4].  The products' operands
 // come from there four columns at a time (rows apart by an odd multiple of 16 bytes: no bank conflicts).  COPIES: f32 rows that are aligned are copied
-// by cp.async, the keys of the next tile behind this one's scores, the values beside them.
+// by cp.async, the keys of the next tile behind this one's scores, the values beside them.  A weight of 0 times an infinite value is NaN: a CTA whose sums are not
+// finite goes through its keys again and leaves the products of rows with keys that they do not see out, one by one, in tiles with such values.
 constexpr int KEYS = 64;
 __device__ __forceinline__ void copy16(float *dst, const float *src, bool valid) {      // zeros if not
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -116,98 +118,144 @@ masked_attention_generic_kernel(Params p) {
 #pragma unroll
     for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
   }
-  for (int tile = first; tile < last; ++tile) {
-    fetch(v, dv, vs, vld, tile);                           // its last readers are behind the barrier at the end of a tile
-    if constexpr (COPIES) copies_wait<1>();                // the keys
-    __syncthreads();
-    float sc[RM][4];
+  auto all_tiles = [&](auto careful) {
+    for (int tile = first; tile < last; ++tile) {
+      fetch(v, dv, vs, vld, tile);                           // its last readers are behind the barrier at the end of a tile
+      if constexpr (COPIES) copies_wait<1>();                // the keys
+      __syncthreads();
+      float sc[RM][4];
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
+      for (int c = 0; c < dq; c += 4) {
+        float4 a[RM], b[4];
+#pragma unroll
+        for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4 *>(qs + (ty * RM + i) * kld + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4 *>(ks + (tx + 16 * j) * kld + c);
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sc[i][j] = fmaf(a[i].x, b[j].x, sc[i][j]);
+            sc[i][j] = fmaf(a[i].y, b[j].y, sc[i][j]);
+            sc[i][j] = fmaf(a[i].z, b[j].z, sc[i][j]);
+            sc[i][j] = fmaf(a[i].w, b[j].w, sc[i][j]);
+          }
+      }
+      // a tile that every row sees whole, as most are, needs no mask
+      const int low = key_of(tile * KEYS), high = key_of(min(tile * KEYS + KEYS, n_keys) - 1);
+      const bool whole = tile * KEYS + KEYS <= n_keys && (TREE ? high < pos : high <= pos + i0 && (low > pos + i1 - p.mask.window || high < p.mask.sinks));
+      auto sees = [&](int i, int place) {                    // row ty * RM + i, a place in the list
+        const int key = key_of(place);
+        bool on;
+        if constexpr (TREE) {
+          const int node = key - pos;
+          on = node < 0 || (node < p.mask.t && (bits[(ty * RM + i) * 4 + (node >> 5)] >> (node & 31) & 1u));
+        } else {
+          on = key <= at[i] && (key > at[i] - p.mask.window || key < p.mask.sinks);
+        }
+        return on && place < n_keys;
+      };
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < RM; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (!sees(i, tile * KEYS + tx + 16 * j)) sc[i][j] = -INFINITY;
+      }
+#pragma unroll
+      for (int i = 0; i < RM; ++i) {
+        float mx = fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3]));
+#pragma unroll
+        for (int e = 8; e > 0; e >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, e));
+        const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn;       // a row may see nothing of this tile
+        const float alpha = ex2(m[i] - base);
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float w = ex2(sc[i][j] - base);
+          sum += w;
+          ps[(ty * RM + i) * PLD + tx + 16 * j] = w;
+        }
+        l[i] = l[i] * alpha + sum;                           // of this thread's keys; added up behind the last tile
+        m[i] = mn;
+#pragma unroll
+        for (int c = 0; c < 4 * NC; ++c) o[i][c] *= alpha;
+      }
+      if constexpr (COPIES) copies_wait<0>();                // the values
+      bool one_by_one = false;
+      if constexpr (careful.value) {
+        if (!whole)
+          for (int r = ty; r < KEYS; r += 16)                // what this thread has copied
+            for (int c = COPIES ? 4 * tx : tx; c < dv; c += COPIES ? 64 : 16)
+#pragma unroll
+              for (int e = 0; e < (COPIES ? 4 : 1); ++e) one_by_one |= !(fabsf(vs[r * vld + c + e]) < INFINITY);
+        one_by_one = __syncthreads_or(one_by_one);
+      } else {
+        __syncthreads();
+      }
+      if (tile + 1 < last) fetch(k, dq, ks, kld, tile + 1);  // the scores are done with the keys
+      if constexpr (careful.value) {
+        if (one_by_one)
+#pragma unroll 1
+          for (int key = 0; key < KEYS; ++key)
+#pragma unroll
+            for (int i = 0; i < RM; ++i) {
+              if (!sees(i, tile * KEYS + key)) continue;
+              const float w = ps[(ty * RM + i) * PLD + key];
+#pragma unroll
+              for (int c = 0; c < 4 * NC; ++c)
+                if (4 * tx + 64 * (c / 4) < dv) o[i][c] = fmaf(w, vs[key * vld + 4 * tx + 64 * (c / 4) + c % 4], o[i][c]);
+            }
+      }
+      for (int key = one_by_one ? KEYS : 0; key < KEYS; key += 4) {
+        float4 w[RM];
+#pragma unroll
+        for (int i = 0; i < RM; ++i) w[i] = *reinterpret_cast<const float4 *>(ps + (ty * RM + i) * PLD + key);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            if (4 * tx + 64 * c >= dv) continue;
+            const float4 b = *reinterpret_cast<const float4 *>(vs + (key + e) * vld + 4 * tx + 64 * c);
+#pragma unroll
+            for (int i = 0; i < RM; ++i) {
+              const float a = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
+              o[i][4 * c] = fmaf(a, b.x, o[i][4 * c]);
+              o[i][4 * c + 1] = fmaf(a, b.y, o[i][4 * c + 1]);
+              o[i][4 * c + 2] = fmaf(a, b.z, o[i][4 * c + 2]);
+              o[i][4 * c + 3] = fmaf(a, b.w, o[i][4 * c + 3]);
+            }
+          }
+      }
+      __syncthreads();
+    }
 #pragma unroll
     for (int i = 0; i < RM; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sc[i][j] = 0.f;
-    for (int c = 0; c < dq; c += 4) {
-      float4 a[RM], b[4];
+      for (int e = 8; e > 0; e >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], e);
+  };
+  all_tiles(std::false_type());
+  bool finite = true;                                      // of rows whose weights are numbers
 #pragma unroll
-      for (int i = 0; i < RM; ++i) a[i] = *reinterpret_cast<const float4 *>(qs + (ty * RM + i) * kld + c);
+  for (int i = 0; i < RM; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const float4 *>(ks + (tx + 16 * j) * kld + c);
-#pragma unroll
-      for (int i = 0; i < RM; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          sc[i][j] = fmaf(a[i].x, b[j].x, sc[i][j]);
-          sc[i][j] = fmaf(a[i].y, b[j].y, sc[i][j]);
-          sc[i][j] = fmaf(a[i].z, b[j].z, sc[i][j]);
-          sc[i][j] = fmaf(a[i].w, b[j].w, sc[i][j]);
-        }
-    }
-    // a tile that every row sees whole, as most are, needs no mask
-    const int low = key_of(tile * KEYS), high = key_of(min(tile * KEYS + KEYS, n_keys) - 1);
-    const bool whole = tile * KEYS + KEYS <= n_keys && (TREE ? high < pos : high <= pos + i0 && (low > pos + i1 - p.mask.window || high < p.mask.sinks));
-    if (!whole) {
-#pragma unroll
-      for (int i = 0; i < RM; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int place = tile * KEYS + tx + 16 * j, key = key_of(place);
-          bool on;
-          if constexpr (TREE) {
-            const int node = key - pos;
-            on = node < 0 || (node < p.mask.t && (bits[(ty * RM + i) * 4 + (node >> 5)] >> (node & 31) & 1u));
-          } else {
-            on = key <= at[i] && (key > at[i] - p.mask.window || key < p.mask.sinks);
-          }
-          if (!(on && place < n_keys)) sc[i][j] = -INFINITY;
-        }
-    }
+    for (int c = 0; c < 4 * NC; ++c) finite = finite && (fabsf(o[i][c]) < INFINITY || l[i] != l[i]);
+  if (__syncthreads_or(!finite)) {
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
-      float mx = fmaxf(fmaxf(sc[i][0], sc[i][1]), fmaxf(sc[i][2], sc[i][3]));
+      m[i] = -INFINITY;
+      l[i] = 0.f;
 #pragma unroll
-      for (int e = 8; e > 0; e >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, e));
-      const float mn = fmaxf(m[i], mx), base = mn == -INFINITY ? 0.f : mn;       // a row may see nothing of this tile
-      const float alpha = ex2(m[i] - base);
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float w = ex2(sc[i][j] - base);
-        sum += w;
-        ps[(ty * RM + i) * PLD + tx + 16 * j] = w;
-      }
-      l[i] = l[i] * alpha + sum;                           // of this thread's keys; added up behind the last tile
-      m[i] = mn;
-#pragma unroll
-      for (int c = 0; c < 4 * NC; ++c) o[i][c] *= alpha;
+      for (int c = 0; c < 4 * NC; ++c) o[i][c] = 0.f;
     }
-    if constexpr (COPIES) copies_wait<0>();                // the values
-    __syncthreads();
-    if (tile + 1 < last) fetch(k, dq, ks, kld, tile + 1);  // the scores are done with the keys
-    for (int key = 0; key < KEYS; key += 4) {
-      float4 w[RM];
-#pragma unroll
-      for (int i = 0; i < RM; ++i) w[i] = *reinterpret_cast<const float4 *>(ps + (ty * RM + i) * PLD + key);
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          if (4 * tx + 64 * c >= dv) continue;
-          const float4 b = *reinterpret_cast<const float4 *>(vs + (key + e) * vld + 4 * tx + 64 * c);
-#pragma unroll
-          for (int i = 0; i < RM; ++i) {
-            const float a = e == 0 ? w[i].x : e == 1 ? w[i].y : e == 2 ? w[i].z : w[i].w;
-            o[i][4 * c] = fmaf(a, b.x, o[i][4 * c]);
-            o[i][4 * c + 1] = fmaf(a, b.y, o[i][4 * c + 1]);
-            o[i][4 * c + 2] = fmaf(a, b.z, o[i][4 * c + 2]);
-            o[i][4 * c + 3] = fmaf(a, b.w, o[i][4 * c + 3]);
-          }
-        }
-    }
-    __syncthreads();
+    fetch(k, dq, ks, kld, first);
+    all_tiles(std::true_type());
   }
 #pragma unroll
   for (int i = 0; i < RM; ++i) {
-#pragma unroll
-    for (int e = 8; e > 0; e >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], e);
     const int r = ty * RM + i, row = row0 + r;
     if (r >= n_rows) continue;
     if (p.splits == 1) {

@@ -41,14 +41,19 @@ __device__ __forceinline__ void raise_invalid(ugb_status_word *status, int detai
   if (atomicCAS(&status->code, 0u, (unsigned)UGB_ERR_INVALID) == 0u) status->detail = (unsigned)detail;
 }
 
-// The keys that rows of queries i0 .. i1 of a sequence see: positions below `first`, and from `from` to `end` - 1.
-struct Span { int first, from, end; };
+// The keys that rows of queries i0 .. i1 of a sequence see: positions below `first`, and from `from` to `end` - 1.  All of the rows see those below `high`
+// that are not below `low`, or that are first positions of the window's mask.
+struct Span { int first, from, end, low, high; };
 template <bool TREE> __device__ __forceinline__ Span span_of(const ugb_mask &m, int pos, int i0, int i1) {
   Span s;
   s.end = pos + i1 + 1;
   s.first = 0;
   s.from = 0;
+  s.low = 0;
+  s.high = pos;
   if constexpr (!TREE) {
+    s.low = max(0, pos + i1 - m.window + 1);
+    s.high = pos + i0 + 1;
     s.from = max(0, pos + i0 - m.window + 1);
     s.first = min(m.sinks, s.from);
   }

@@ -12,7 +12,10 @@
 // it was last (the probabilities are then up to 2^8, which costs bf16 no precision, and the sum is f32), which after the first tiles is hardly ever.
 // Up to 32 rows (single positions, small trees) lie four times in the tile, once for each softmax warp, which takes a quarter of every tile's keys: a
 // warp's chain per tile is then short enough for HBM.  The quarters are joined as slices of the keys are, by the combine kernel.
-// Results leave through shared memory, by TMA.  Rows of V that no row of the item sees are set to zero there: P is zero for them, but 0 x NaN is not.
+// Results leave through shared memory, by TMA.  Rows of V that no row of the item sees are set to zero there: P is zero for them, but 0 x NaN is not.  So is what
+// is not finite in rows that only some see; those get it behind the last tile, from memory.  With two groups the warps that are left of the first
+// warpgroup do this, while the tile's softmax is on its way (4 x 2048 positions as below 209 us for 204 without looking for what is not finite); a tile
+// looked through by the softmax warps of the first group 211 us, and one of single positions, all of them, 68 us for 56.
 // Grid: one CTA per item; a CTA that is done takes over the item of one that has not started (cluster launch control), so that its set-up and its
 // TMEM are shared by many and long and short items even out.  Every wait on an mbarrier is bounded.
 //
@@ -43,7 +46,7 @@ constexpr int P_BYTES = 2 * BLOCK;                         // 128 rows x 128 key
 // RT 0: up to 32 rows, spread over the four warps of one group.
 template <int DQ, int DV, int RT0> struct Shape {
   static constexpr int RT = RT0 ? RT0 : 1;
-  // Two groups: the softmax warps are two whole warpgroups, which take registers over from the first one (two of its warps have no part).
+  // Two groups: the softmax warps are two whole warpgroups, which take registers over from the first one.
   static constexpr int FIRST = RT == 2 ? 4 : 2, THREADS = 32 * FIRST + 128 * RT;    // FIRST: softmax warp
   static constexpr int Q_BYTES = DQ / CB * BLOCK, STAGE = (DQ > DV ? DQ : DV) / CB * BLOCK;     // a stage holds a tile of keys or of values
   static constexpr int O_COL = RT * KEYS;                  // TMEM: S [RT][128], then O [RT][DV]
@@ -133,6 +136,43 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap *map, uint32_t sr
 __device__ __forceinline__ void store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void store_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// Row `row` of a tile of values, whose key not all rows of the item see: zeros, or zeros for what is not finite.  Whether there was any of that.
+template <int DV> __device__ __forceinline__ bool clean_values(uint8_t *stage, int row, bool nobody) {
+  uint8_t *const at = stage + row * 128;                   // 16 bytes at a time, others first in every row: no bank conflicts
+  if (nobody) {
+#pragma unroll
+    for (int x = 0; x < DV / 8; ++x) *reinterpret_cast<uint4 *>(at + x / 8 * BLOCK + ((x ^ row) & 7) * 16) = make_uint4(0, 0, 0, 0);
+    return false;
+  }
+  const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
+  __nv_bfloat162 sum = zero;                               // of 0 x value: NaN if any is not finite
+#pragma unroll
+  for (int x = 0; x < DV / 8; ++x) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(at + x / 8 * BLOCK + ((x ^ row) & 7) * 16);
+    const __nv_bfloat162 *w = reinterpret_cast<const __nv_bfloat162 *>(&v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum = __hfma2(w[e], zero, sum);
+  }
+  const uint32_t bits = *reinterpret_cast<const uint32_t *>(&sum);
+  if (!(bits & 0x7fff7fffu)) return false;
+#pragma unroll 1
+  for (int x = 0; x < DV; ++x) {
+    uint16_t *v = reinterpret_cast<uint16_t *>(at + x / 64 * BLOCK) + x % 64;
+    if ((*v & 0x7f80) == 0x7f80) *v = 0;
+  }
+  return true;
+}
+// What is not finite in columns c .. c + 31 of the keys of `seen`, v: the values of its first key.  Hardly ever called.
+struct NotFinite { uint32_t plus, minus, nan; };
+__device__ __noinline__ NotFinite not_finite(const uint16_t *v, int dv, int c, unsigned long long seen) {
+  NotFinite r{0, 0, 0};
+  for (; seen; seen &= seen - 1) {
+    const uint16_t *x = v + (size_t)(__ffsll((long long)seen) - 1) * dv + c;
+    for (int e = 0; e < min(32, dv - c); ++e)
+      if ((x[e] & 0x7f80) == 0x7f80) (x[e] & 0x7f ? r.nan : x[e] & 0x8000 ? r.minus : r.plus) |= 1u << e;
+  }
+  return r;
+}
 // The lowest n bits, n clamped to 0 .. 64.
 __device__ __forceinline__ unsigned long long low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
@@ -147,6 +187,11 @@ struct Item {
   __device__ __forceinline__ bool full(int j) const {      // the last of the first tiles may hold the start of the window too
     return (first + j < first_tiles && span.from >= first_tiles * KEYS ? span.first : span.end) - key0(j) > 64;
   }
+  // which of the item's stages holds the values of tile j: K(0), then K(j + 1), V(j) for every tile, and V of the last one
+  __device__ __forceinline__ int stage_of_values(int j) const { return j + 1 < tiles ? 2 * j + 2 : 2 * j + 1; }
+  __device__ __forceinline__ bool nobody_sees(int k) const { return k >= span.first && (k < span.from || k >= span.end); }
+  // whether all rows see the keys from k on, n of them
+  __device__ __forceinline__ bool all_see(int k, int n, int sinks) const { return k + n <= span.high && (k >= span.low || k + n <= sinks); }
 };
 template <int RT, bool TREE> __device__ __forceinline__ Item item_of(int idx, const Params &p) {
   Item it;
@@ -187,11 +232,12 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
   uint64_t *bars = (uint64_t *)(kv_s + ST * Sh::STAGE);
   uint64_t *q_full = bars, *q_empty = bars + 1, *answer_full = bars + 2, *answer = bars + 4;       // the answer: 16 bytes, aligned
   uint64_t *item_full = bars + 6, *item_empty = bars + 8, *s_full = bars + 10, *s_free = s_full + RT, *p_full = s_free + RT, *o_full = p_full + RT;
-  uint64_t *kv_full = o_full + RT, *kv_empty = kv_full + ST;
-  uint32_t *tmem_slot = (uint32_t *)(kv_empty + ST);
+  uint64_t *kv_full = o_full + RT, *kv_empty = kv_full + ST, *v_ready = kv_empty + ST, *v_clean = v_ready + 1;
+  uint32_t *tmem_slot = (uint32_t *)(v_clean + 1);
   volatile int *abort_flag = (volatile int *)(tmem_slot + 1), *item_slot = (volatile int *)(tmem_slot + 2);      // two entries
+  volatile int *not_finite_slot = item_slot + 2;           // four: the items since which values were set to zero, one more than their number
   int(*up)[UGB_TREE_MAX] = (int(*)[UGB_TREE_MAX])((uint8_t *)bars + 512);
-  static_assert((10 + 4 * RT + 2 * ST) * 8 + 16 <= 512, "barriers fit");
+  static_assert((12 + 4 * RT + 2 * ST) * 8 + 32 <= 512, "barriers fit");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   ugb_status_word *const status = p.m.status;
@@ -201,7 +247,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
     mbar_init(smem_u32(answer_full), 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&item_full[i]), 1);
-      mbar_init(smem_u32(&item_empty[i]), 1 + 4 * RT);
+      mbar_init(smem_u32(&item_empty[i]), 1 + 4 * RT + (RT == 2 ? 2 : 0));
     }
     for (int i = 0; i < RT; ++i) {
       mbar_init(smem_u32(&s_full[i]), 1);
@@ -213,7 +259,10 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
       mbar_init(smem_u32(&kv_full[i]), 1);
       mbar_init(smem_u32(&kv_empty[i]), 1);
     }
+    mbar_init(smem_u32(v_ready), 1);
+    mbar_init(smem_u32(v_clean), 2);
     *abort_flag = 0;
+    for (int i = 0; i < 4; ++i) not_finite_slot[i] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmQ) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&tmK) : "memory");
@@ -295,6 +344,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
       const uint64_t k_desc = make_smem_desc(smem_u32(kv_s), 0, 1024), v_desc = make_smem_desc(smem_u32(kv_s), BLOCK, 1024);
       int g = 0, n_q = 0;                                               // stages and items so far
       uint32_t n_s[2] = {0, 0}, n_p[2] = {0, 0};                        // S and P V products of a group so far
+      uint32_t n_clean = 0;                                             // tiles of values that were cleaned so far
       for (int n_it = 0;; ++n_it) {
         const int at = n_it & 1;
         if (!mbar_wait(smem_u32(&item_full[at]), (uint32_t)(n_it >> 1) & 1u, abort_flag, status, 0x65)) break;
@@ -340,6 +390,11 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
           ++g;
           const uint64_t vd = v_desc + (uint64_t)(s * (Sh::STAGE >> 4));
           const bool full = it.full(j);
+          if (RT == 2 && !it.all_see(it.key0(j), full ? KEYS : 64, p.m.mask.sinks)) {
+            mbar_arrive(smem_u32(v_ready));
+            if (!mbar_wait(smem_u32(v_clean), n_clean & 1u, abort_flag, status, 0x63)) { alive = false; break; }
+            ++n_clean;
+          }
 #pragma unroll
           for (int a = 0; a < RT; ++a) {
             if (a == 1 && !both) break;
@@ -360,6 +415,39 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
         }
         if (!alive) break;
       }
+    }
+  } else if (RT == 2) {
+    // ------------------------------------------- values of keys that not all rows see --
+    // While the softmax of the tile is on its way.  The issuer says when a tile is there: a wait for a stage that it has not got to might take an older phase of its
+    // barrier for the one that is meant.
+    bool alive = true;
+    int g0 = 0;                                            // stages of the CTA so far
+    uint32_t n_clean = 0;
+    for (int n_it = 0; alive; ++n_it) {
+      const int at = n_it & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&item_full[at]), (uint32_t)(n_it >> 1) & 1u, abort_flag, status, 0x6b))) break;
+      const int idx = item_slot[at];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&item_empty[at]));
+      if (idx < 0) break;
+      const Item it = item_of<RT, TREE>(idx, p);
+      for (int j = 0; j < it.tiles; ++j) {
+        const int key0 = it.key0(j), n_keys = it.full(j) ? KEYS : 64;
+        if (it.all_see(key0, n_keys, p.m.mask.sinks)) continue;
+        const int g = g0 + it.stage_of_values(j), s = g % ST;
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(v_ready), n_clean & 1u, abort_flag, status, 0x6e) &&
+                                         mbar_wait(smem_u32(&kv_full[s]), (uint32_t)(g / ST) & 1u, abort_flag, status, 0x6e))) { alive = false; break; }
+        ++n_clean;
+        for (int row = threadIdx.x - 64; row < n_keys; row += 64) {
+          const bool nobody = it.nobody_sees(key0 + row);
+          if ((nobody || !it.all_see(key0 + row, 1, p.m.mask.sinks)) && clean_values<DV>(kv_s + s * Sh::STAGE, row, nobody))
+            not_finite_slot[n_it & 3] = n_it + 1;          // the groups are two items behind at most
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(v_clean));
+      }
+      g0 += 2 * it.tiles;
     }
   }
   } else {
@@ -583,15 +671,14 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
             group_sync(1 + a);
           }
         }
-        // keys of the tile that no row of the item sees: their values may be anything
-        const int n_keys = full ? KEYS : 64;
-        if (a == 0 && !(key0 + n_keys <= it.span.first || (key0 >= it.span.from && key0 + n_keys <= it.span.end))) {
-          const int g = g0 + (j + 1 < it.tiles ? 2 * j + 2 : 2 * j + 1), s = g % ST;     // stage of V(j)
-          if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&kv_full[s]), (uint32_t)(g / ST) & 1u, abort_flag, status, 0x6e))) { alive = false; break; }
-          for (int x = row; x < KEYS * (DV / 8); x += 128) {
-            const int key = key0 + x % KEYS;
-            if (x % KEYS < n_keys && key >= it.span.first && (key < it.span.from || key >= it.span.end))
-              *reinterpret_cast<uint4 *>(kv_s + s * Sh::STAGE + (x / KEYS / 8) * BLOCK + (x % KEYS) * 128 + (x / KEYS % 8) * 16) = make_uint4(0, 0, 0, 0);
+        if constexpr (RT == 1) {                           // with two groups, the warps beside the issuer do this
+          const int n_keys = full ? KEYS : 64;
+          if (!it.all_see(key0, n_keys, p.m.mask.sinks)) {
+            const int g = g0 + it.stage_of_values(j), s = g % ST;
+            if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&kv_full[s]), (uint32_t)(g / ST) & 1u, abort_flag, status, 0x6e))) { alive = false; break; }
+            const bool nobody = it.nobody_sees(key0 + row);
+            if (row < n_keys && (nobody || !it.all_see(key0 + row, 1, p.m.mask.sinks)) && clean_values<DV>(kv_s + s * Sh::STAGE, row, nobody))
+              not_finite_slot[n_it & 3] = n_it + 1;
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");    // visible to the tensor core's reads
@@ -607,6 +694,42 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
         ++n_o;
         tcgen05_fence_after();
       }
+      const bool zeroed = it.tiles > 0 && not_finite_slot[n_it & 3] == n_it + 1;
+      // what was set to zero of values that this row sees, whose weights are above 0.  SPREAD: the other quarters' keys have weights of 0 in this row, too, so that
+      // an infinite value that all see is NaN here, and has to be infinite in its quarter and to count nothing in the others.
+      auto add_not_finite = [&](uint32_t (&o)[32], int c) {
+        bool add = zeroed;
+        if constexpr (SPREAD) {
+          float any = 0.f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) any = fmaf(__uint_as_float(o[e]), 0.f, any);
+          add = zeroed || __any_sync(0xffffffffu, any != 0.f && l == l);
+        }
+        if (!add) return;
+        NotFinite all{0, 0, 0};
+        const uint16_t *v = (const uint16_t *)p.m.v + ((size_t)it.s * p.m.kv_heads + it.kvh) * p.m.mask.t_max * p.m.dv;
+        for (int j = 0; j < it.tiles; ++j) {
+          const int key0 = it.key0(j), halves = it.full(j) ? 2 : 1;
+          if (!SPREAD && it.all_see(key0, 64 * halves, p.m.mask.sinks)) continue;
+          for (int h = 0; h < halves; ++h) {
+            unsigned long long seen = seen_from(key0 + 64 * h);
+            if (SPREAD) seen &= quad / 2 == h ? 0xffffffffull << (32 * (quad & 1)) : 0ull;
+            const NotFinite r = not_finite(v + (size_t)(key0 + 64 * h) * p.m.dv, p.m.dv, c, seen);
+            all.plus |= r.plus;
+            all.minus |= r.minus;
+            all.nan |= r.nan;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          float x = __uint_as_float(o[e]);
+          if (SPREAD && l == l && x != x) x = 0.f;
+          if (all.plus >> e & 1u) x += INFINITY;
+          if (all.minus >> e & 1u) x -= INFINITY;
+          if (all.nan >> e & 1u) x = NAN;
+          o[e] = __float_as_uint(x);
+        }
+      };
       if (!SPREAD && p.m.splits == 1) {
         // every item has tiles then; the probabilities' buffer takes the result, a block of 64 columns after the other
         const float scale = p.m.out_scale / l;             // at least 1: a row sees itself; 0 where all its scores are -inf, which gives NaN
@@ -616,6 +739,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
             uint32_t o[32];
             tmem_ld_32x32b_x32(o_base + c, o);
             tmem_ld_wait();
+            add_not_finite(o, c);
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
               uint32_t w[4];
@@ -646,6 +770,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
             uint32_t o[32];
             tmem_ld_32x32b_x32(o_base + c, o);
             tmem_ld_wait();
+            add_not_finite(o, c);
             if (write) {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
