@@ -235,7 +235,7 @@ masked_attention_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid
   uint64_t *kv_full = o_full + RT, *kv_empty = kv_full + ST, *v_ready = kv_empty + ST, *v_clean = v_ready + 1;
   uint32_t *tmem_slot = (uint32_t *)(v_clean + 1);
   volatile int *abort_flag = (volatile int *)(tmem_slot + 1), *item_slot = (volatile int *)(tmem_slot + 2);      // two entries
-  volatile int *not_finite_slot = item_slot + 2;           // four: the items since which values were set to zero, one more than their number
+  volatile int *not_finite_slot = item_slot + 2;           // of four items in turn: n_it + 1 where values were set to zero
   int(*up)[UGB_TREE_MAX] = (int(*)[UGB_TREE_MAX])((uint8_t *)bars + 512);
   static_assert((12 + 4 * RT + 2 * ST) * 8 + 32 <= 512, "barriers fit");
 
